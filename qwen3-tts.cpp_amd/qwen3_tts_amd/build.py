@@ -20,7 +20,8 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-SRC_FLAGS = {"q3t_dev.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "q3t_voc.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+SRC_FLAGS = {"q3t_dev.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"], "q3t_voc.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+             "q3t_kv8.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
 
 
 def _run(cmd, verbose):
