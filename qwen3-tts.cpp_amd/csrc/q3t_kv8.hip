@@ -168,22 +168,50 @@ static int check_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     return 0;
 }
 
+// How a call runs: its kernels, splits and the parts of its workspace (bytes).
+struct AttendPlan {
+    bool few;
+    int split_tiles, n_split, score_len;
+    int64_t part, stat, score, total;
+};
+
+static AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
+    AttendPlan p{};
+    const int64_t len = a->max_len ? a->max_len : c->n_slots, heads = (int64_t) c->n_seq * c->n_kv_head;
+    const int64_t group = a->n_head / c->n_kv_head, rows = a->n_rows * group, tiles = (len + 63) / 64;
+    p.few = rows <= (a->weights ? 8 : 32);
+    if (!p.few) {
+        p.total = heads * group * a->n_rows * len * 4;
+        return p;
+    }
+    // 4 tiles (one a wave) to 32 a split, so that there are about 1,024 workgroups: four a CU
+    p.split_tiles = (int) std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 32) + 3 & ~3;
+    p.n_split = (int) ((tiles + p.split_tiles - 1) / p.split_tiles);
+    p.score_len = (int) (tiles * 64);
+    auto take = [&](int64_t bytes) { const int64_t at = p.total; p.total += (bytes + 255) / 256 * 256; return at; };
+    if (p.n_split > 1) p.part = take(heads * p.n_split * rows * c->head_dim * 4);
+    if (p.n_split > 1 || a->weights) p.stat = take(heads * p.n_split * rows * 8);
+    if (a->weights) p.score = take(heads * rows * p.score_len * 4);
+    return p;
+}
+
 int64_t q3t_kv8_attend_ws(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     t_err[0] = 0;
     if (check_attend(c, a)) return -1;
-    const int64_t len = a->max_len ? a->max_len : c->n_slots;
-    return (int64_t) c->n_seq * a->n_head * a->n_rows * len * 4;
+    return plan_attend(c, a).total;
 }
 
 int q3t_kv8_attend(int32_t device, const q3t_kv8 * c, const q3t_kv8_attend_args * p, void * ws, int64_t ws_bytes,
                    void * stream) {
-    const int64_t need = q3t_kv8_attend_ws(c, p);
-    if (need < 0) return -1;
+    t_err[0] = 0;
+    if (check_attend(c, p)) return -1;
     if (!p->n_rows) return 0;
     if (!p->q || !p->out) return refuse("null rows");
-    if (need > 0 && (!ws || ws_bytes < need)) return refuse("workspace too small");
+    const AttendPlan plan = plan_attend(c, p);
+    if (plan.total > 0 && (!ws || ws_bytes < plan.total)) return refuse("workspace too small");
     if (!is16(ws)) return refuse("workspace must be 16-byte aligned");
     ON_DEVICE(device);
+    const hipStream_t st = (hipStream_t) stream;
     kv8::AttendArgs a{};
     a.c = *c; a.q = p->q; a.o = p->out;
     a.qs = p->q_seq; a.qr = p->q_row; a.qh = p->q_head; a.os = p->o_seq; a.orow = p->o_row; a.oh = p->o_head;
@@ -191,12 +219,34 @@ int q3t_kv8_attend(int32_t device, const q3t_kv8 * c, const q3t_kv8_attend_args 
     a.n_rows = p->n_rows; a.n_head = p->n_head; a.group = p->n_head / c->n_kv_head;
     a.max_len = p->max_len ? p->max_len : c->n_slots;
     a.causal = p->causal != 0; a.weights = p->weights != 0; a.scale = p->scale; a.ws = (float *) ws;
+    a.qvec = is16(p->q) && strides16(p->q_type, {p->q_seq, p->q_row, p->q_head});
+    if (plan.few) {
+        a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.score_len = plan.score_len;
+        if (plan.n_split > 1) a.part = (float *) ((char *) ws + plan.part);
+        if (plan.n_split > 1 || a.weights) a.stat = (float2 *) ((char *) ws + plan.stat);
+        if (a.weights) a.score = (float *) ((char *) ws + plan.score);
+        const int rows = a.n_rows * a.group;
+        const dim3 grid(plan.n_split, c->n_kv_head, c->n_seq);
+        if (c->head_dim == 64) {
+            if (rows <= 16) hipLaunchKernelGGL((kv8::k_attend_few<64, 1>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((kv8::k_attend_few<64, 2>), grid, dim3(256), 0, st, a);
+        } else {
+            if (rows <= 16) hipLaunchKernelGGL((kv8::k_attend_few<128, 1>), grid, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL((kv8::k_attend_few<128, 2>), grid, dim3(256), 0, st, a);
+        }
+        const int blocks = (plan.n_split > 1 ? rows : 0) + (a.weights ? (a.max_len + 1023) / 1024 : 0);
+        if (blocks) {
+            const dim3 jg(blocks, c->n_kv_head, c->n_seq);
+            if (c->head_dim == 64) hipLaunchKernelGGL(kv8::k_attend_join<64>, jg, dim3(256), 0, st, a);
+            else hipLaunchKernelGGL(kv8::k_attend_join<128>, jg, dim3(256), 0, st, a);
+        }
+        return launched("attend");
+    }
     const dim3 grid(p->n_rows, p->n_head, c->n_seq);
-    if (c->head_dim == 64) hipLaunchKernelGGL(kv8::k_attend_row<64>, grid, dim3(256), 0, (hipStream_t) stream, a);
-    else hipLaunchKernelGGL(kv8::k_attend_row<128>, grid, dim3(256), 0, (hipStream_t) stream, a);
+    if (c->head_dim == 64) hipLaunchKernelGGL(kv8::k_attend_row<64>, grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(kv8::k_attend_row<128>, grid, dim3(256), 0, st, a);
     if (a.weights)
-        hipLaunchKernelGGL(kv8::k_attend_acc, dim3((a.max_len + 255) / 256, c->n_kv_head, c->n_seq), dim3(256), 0,
-                           (hipStream_t) stream, a);
+        hipLaunchKernelGGL(kv8::k_attend_acc, dim3((a.max_len + 255) / 256, c->n_kv_head, c->n_seq), dim3(256), 0, st, a);
     return launched("attend");
 }
 

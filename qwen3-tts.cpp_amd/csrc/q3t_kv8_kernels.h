@@ -276,6 +276,9 @@ struct AttendArgs {
     int32_t len0, q_type, o_type, n_rows, n_head, group, max_len, causal, weights, qvec, ovec;
     float scale;
     float * ws;
+    // few rows (k_attend_few, k_attend_join)
+    int32_t split_tiles, n_split, score_len;   // 64-slot tiles a split; scores a row
+    float * part; float2 * stat; float * score; // [seq][kv head][split][row][D], [..][row], [seq][kv head][row][score_len]
 };
 
 __device__ __forceinline__ int seq_len(const AttendArgs & a, int s) {
@@ -373,6 +376,353 @@ __global__ __launch_bounds__(256) void k_attend_acc(AttendArgs a) {
             w += exp2f(a.ws[(((int64_t) s * a.n_head + g * a.group + e) * a.n_rows + i) * a.max_len + j]);
     }
     a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += w;
+}
+
+// ------------------------------------------------ attention of a few rows
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+
+// Codes as fp16.  A code's byte with its top bit turned, under the high byte
+// 0x64, is the half 1024 + (code + 128); minus 1152 that is the code, exactly.
+__device__ __forceinline__ uint32_t halves(uint32_t biased, uint32_t sel) {
+    const h2v x = __builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, biased, sel));
+    return __builtin_bit_cast(uint32_t, x + (h2v){(_Float16) -1152, (_Float16) -1152});
+}
+constexpr uint32_t kSelLo = 0x04010400u, kSelHi = 0x04030402u;   // bytes 0, 1 or 2, 3 of a word, each under 0x64
+__device__ __forceinline__ h8v halves8(uint32_t a, uint32_t b) {
+    a ^= 0x80808080u;
+    b ^= 0x80808080u;
+    const i4 v = {(int) halves(a, kSelLo), (int) halves(a, kSelHi), (int) halves(b, kSelLo), (int) halves(b, kSelHi)};
+    return __builtin_bit_cast(h8v, v);
+}
+__device__ __forceinline__ f4 mfma32(h8v a, h8v b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ uint32_t pack_h(float a, float b) {
+    const h2v v = {(_Float16) a, (_Float16) b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// One row of q as MFMA operands: lane group k = l / 16 holds dims (D / 4) k + 8 c .. + 7 in q[c], in fp16 under the power
+// of two that brings the row's largest value to [1, 2) (exact for fp16 and for all bits of bfloat16 values down to
+// 2^-14 of the largest).  Returns what a product with it is to be multiplied by, NaN for a row that is not finite.
+template <int D>
+__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, h8v (&q)[D / 32]) {
+    float x[D / 32][8], big = 0.0f, ok = 0.0f;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
+        if (on) {
+            if (a.q_type == kF16) load8<kF16>(a.q, at + 8 * c, a.qvec, x[c]);
+            else load8<kBF16>(a.q, at + 8 * c, a.qvec, x[c]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            big = fmaxf(big, fabsf(x[c][e]));
+            ok = fmaf(x[c][e], 0.0f, ok);       // NaN once a value is not finite
+        }
+    }
+    big = fmaxf(big, __shfl_xor(big, 16));
+    big = fmaxf(big, __shfl_xor(big, 32));
+    ok += __shfl_xor(ok, 16);
+    ok += __shfl_xor(ok, 32);
+    const int ex = big > 0.0f && finite_f(big) ? ilogbf(big) : 0;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) q[c][e] = (_Float16) ldexpf(x[c][e], -ex);
+    return ldexpf(a.scale * 1.4426950408889634f, ex) + ok;
+}
+
+constexpr float kPScale = 16384.0f;    // probabilities enter the value product times this (fp16's normal range then ends at 2^-28)
+
+// Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (splits, kv heads, sequences), four
+// waves.  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its own running
+// maximum m and sum, and join at the end.
+//   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16,
+//     k = l / 16) holds dims (D / 4) k .. of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
+//   - O^T = V^T . P^T: those probabilities are the B operand where they lie, if the 32 slots of an MFMA
+//     are taken as 4k + e of one block of 16, then of the next; lane (i, k) then needs the codes of dims (D / 16) i .. of
+//     those slots, which it reads as one piece of a row, and turns round by byte permutations while they
+//     become halves.  Row i's dims (D / 4) k .. are its outputs.
+//   - Codes are exact in fp16; a key block's scale multiplies its scores, a value block's the probabilities, under
+//     the largest value scale so far (vref) and kPScale, so that they neither overflow nor lose bits.
+//   - With several splits each writes m, the sum and its unnormalised rows; k_attend_join puts them together.
+template <int D, int RT>
+__global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
+    constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
+    __shared__ float mo[4][16][LD], mm[4][16], ml[4][16];
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
+    const int g = blockIdx.y, s = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
+    const int tiles = (len + 63) / 64, t0 = blockIdx.x * a.split_tiles, t1 = min(t0 + a.split_tiles, tiles);
+    if (!n || (blockIdx.x && t0 >= tiles)) return;
+    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + (D / 4) * k, * vb = a.c.v + s * a.c.seq + g * a.c.head + NJ * i;
+    const float * sb = (l & 4 ? a.c.vs : a.c.ks) + s * a.c.scale_seq + g * a.c.scale_head;
+    const int last = len - 1, last_blk = last / kBlk;
+    float * sco = a.score ? a.score + ((int64_t) s * a.c.n_kv_head + g) * a.n_rows * a.group * a.score_len : nullptr;
+
+    u4 kr[4][D / 64];
+    uint32_t vr[16][NJ / 4];
+    float sr;
+    auto fetch_k = [&](int tile) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int8_t * p = kb + (int64_t) min(tile * 64 + 16 * b + i, last) * D;
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c) kr[b][c] = *(const u4 *) (p + 16 * c);
+        }
+        const int blk = tile * 4 + (l & 3);
+        sr = sb[min(blk, last_blk)];
+        if (blk > last_blk) sr = 0.0f;
+    };
+    auto fetch_v = [&](int tile) {
+#pragma unroll
+        for (int b = 0; b < 4; ++b)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int8_t * p = vb + (int64_t) min(tile * 64 + 16 * b + 4 * k + e, last) * D;
+                if constexpr (D == 128) {
+                    const u2 x = *(const u2 *) p;
+                    vr[4 * b + e][0] = x[0];
+                    vr[4 * b + e][1] = x[1];
+                } else {
+                    vr[4 * b + e][0] = *(const uint32_t *) p;
+                }
+            }
+    };
+    const int first = t0 + w;
+    if (first < t1) {
+        fetch_k(first);
+        fetch_v(first);
+    }
+    h8v q[RT][NC];
+    float qs[RT], m[RT], sum[RT], vref = 0.0f;
+    int lim[RT];
+    f4 o[RT][NJ];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = 16 * r + i;
+        const bool on = row < rows;
+        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qh + (D / 4) * k, on, q[r]);
+        lim[r] = on ? row_limit(a, len, n, tok) : 0;
+        m[r] = -INFINITY;
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
+    }
+    const int lim_all = row_limit(a, len, n, 0);    // slots that every row sees
+    for (int tile = first; tile < t1; tile += 4) {
+        f4 sc[RT][4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+#pragma unroll
+            for (int r = 0; r < RT; ++r) sc[r][b] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const h8v kf = halves8(kr[b][c / 2][2 * (c & 1)], kr[b][c / 2][2 * (c & 1) + 1]);
+#pragma unroll
+                for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf, q[r][c], sc[r][b]);
+            }
+        }
+        float ks[4], vs[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sr), b));
+            vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sr), 4 + b));
+        }
+        if (tile + 4 < t1) fetch_k(tile + 4);
+        const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+        const float vnew = fmaxf(vref, vtop), vscale = vnew > 0.0f ? kPScale / vnew : 0.0f;
+        const float vmove = vnew > vref ? vref / vnew : 1.0f;
+        vref = vnew;
+        h8v p[RT][2];
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            float top = -INFINITY;
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                sc[r][b] *= ks[b] * qs[r];
+                if (tile * 64 + 63 >= lim_all)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        sc[r][b][e] = tile * 64 + 16 * b + 4 * k + e < lim[r] ? sc[r][b][e] : -INFINITY;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[r][b][e]);
+            }
+            if (sco && 16 * r + i < rows)
+#pragma unroll
+                for (int b = 0; b < 4; ++b)
+                    *(f4 *) (sco + (int64_t) (16 * r + i) * a.score_len + tile * 64 + 16 * b + 4 * k) = sc[r][b];
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(top, __shfl_xor(top, 32));
+            const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
+            const float move = __builtin_amdgcn_exp2f(m[r] - base);     // 0 at first
+            if (__any(mn > m[r]) || vmove != 1.0f) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[r][j] *= move * vmove;
+            }
+            m[r] = mn;
+            float add = 0.0f;
+            uint32_t pw[4][2];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                float x[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
+                    add += x[e];
+                    x[e] *= vs[b] * vscale;
+                }
+                pw[b][0] = pack_h(x[0], x[1]);
+                pw[b][1] = pack_h(x[2], x[3]);
+            }
+            sum[r] = fmaf(sum[r], move, add);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const i4 v = {(int) pw[2 * u][0], (int) pw[2 * u][1], (int) pw[2 * u + 1][0], (int) pw[2 * u + 1][1]};
+                p[r][u] = __builtin_bit_cast(h8v, v);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int d = 0; d < NJ / 4; ++d) {
+                uint32_t f[4][4];                   // dims 4d .. 4d + 3 of this lane: slots in pairs
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t w0 = vr[8 * u + 2 * x][d] ^ 0x80808080u, w1 = vr[8 * u + 2 * x + 1][d] ^ 0x80808080u;
+                    const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+                    f[0][x] = halves(lo, kSelLo);
+                    f[1][x] = halves(lo, kSelHi);
+                    f[2][x] = halves(hi, kSelLo);
+                    f[3][x] = halves(hi, kSelHi);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const i4 v = {(int) f[j][0], (int) f[j][1], (int) f[j][2], (int) f[j][3]};
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) o[r][4 * d + j] = mfma32(__builtin_bit_cast(h8v, v), p[r][u], o[r][4 * d + j]);
+                }
+            }
+        if (tile + 4 < t1) fetch_v(tile + 4);
+    }
+    // the four waves' rows under their common maximum, added in wave order
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        sum[r] += __shfl_xor(sum[r], 16);
+        sum[r] += __shfl_xor(sum[r], 32);
+        if (r) __syncthreads();
+        if (k == 0) { mm[w][i] = m[r]; ml[w][i] = sum[r]; }
+        __syncthreads();
+        const float top = fmaxf(fmaxf(mm[0][i], mm[1][i]), fmaxf(mm[2][i], mm[3][i])), base = top == -INFINITY ? 0.0f : top;
+        const float f = __builtin_amdgcn_exp2f(m[r] - base) * (vref / kPScale);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int j = 0; j < NJ; j += 4)
+                *(f4 *) &mo[w][i][(D / 4) * k + NJ * e + j] = (f4){o[r][j][e], o[r][j + 1][e], o[r][j + 2][e], o[r][j + 3][e]} * f;
+        __syncthreads();
+        const int row = t >> 4, d0 = (t & 15) * NJ, at = 16 * r + row;
+        const float big = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
+        float all = 0.0f;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) all += ml[x][row] * __builtin_amdgcn_exp2f(mm[x][row] - (big == -INFINITY ? 0.0f : big));
+        if (at < rows) {
+            const int64_t cell = (((int64_t) s * a.c.n_kv_head + g) * a.n_split + blockIdx.x) * a.n_rows * a.group + at;
+            if (a.stat && d0 == 0) a.stat[cell] = make_float2(big, all);
+            const float inv = a.n_split > 1 ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
+            float y[8];
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) y[j] = (((mo[0][row][d0 + j] + mo[1][row][d0 + j]) + mo[2][row][d0 + j]) + mo[3][row][d0 + j]) * inv;
+            if (a.n_split > 1) {
+#pragma unroll
+                for (int j = 0; j < NJ; j += 4) *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
+            } else {
+                const int64_t out = s * a.os + at / a.group * a.orow + (g * a.group + at % a.group) * a.oh + d0;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) {
+                    if (a.o_type == kF32) ((float *) a.o)[out + j] = y[j];
+                    else ((uint16_t *) a.o)[out + j] = a.o_type == kF16 ? f2h(y[j]) : f2bf(y[j]);
+                }
+            }
+        }
+    }
+}
+
+// grid (rows if split, then slots / 1024 if weights are kept; kv heads; sequences).  A row's splits put together: D / 4
+// lanes by 1024 / D groups of splits, the groups added in order; or acc of 1,024 slots from the kept scores.
+template <int D>
+__global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
+    constexpr int LN = D / 4, GR = 256 / LN;
+    __shared__ f4 po[GR][LN];
+    __shared__ float pl[GR], lse[8];
+    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
+    const int live = min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
+    const int64_t head = (int64_t) s * a.c.n_kv_head + g;
+    const int nr = a.n_split > 1 ? all_rows : 0;
+    if ((int) blockIdx.x < nr) {
+        const int row = blockIdx.x, gr = t / LN, ln = t % LN;
+        if (row >= rows) return;
+        const int64_t cell = head * a.n_split * all_rows + row;
+        float top = -INFINITY;
+        for (int x = 0; x < live; ++x) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
+        const float base = top == -INFINITY ? 0.0f : top;
+        f4 o = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.0f;
+        for (int x = gr; x < live; x += GR) {
+            const int64_t at = cell + (int64_t) x * all_rows;
+            const float2 st = a.stat[at];
+            const float f = __builtin_amdgcn_exp2f(st.x - base);
+            o += *(const f4 *) (a.part + at * D + 4 * ln) * f;
+            sum = fmaf(st.y, f, sum);
+        }
+        po[gr][ln] = o;
+        if (ln == 0) pl[gr] = sum;
+        __syncthreads();
+        if (gr) return;
+#pragma unroll
+        for (int x = 1; x < GR; ++x) {
+            o += po[x][ln];
+            sum += pl[x];
+        }
+        o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int64_t out = s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * ln;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (a.o_type == kF32) ((float *) a.o)[out + e] = o[e];
+            else ((uint16_t *) a.o)[out + e] = a.o_type == kF16 ? f2h(o[e]) : f2bf(o[e]);
+        }
+        return;
+    }
+    const int j0 = (blockIdx.x - nr) * 1024;
+    if (j0 >= len || !n) return;
+    for (int r = t >> 6; r < rows; r += 4) {        // one wave a row: log2 of the row's sum of exponentials
+        const int64_t cell = head * a.n_split * all_rows + r;
+        float top = -INFINITY, sum = 0.0f;
+        for (int x = t & 63; x < live; x += 64) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
+        top = wave_max_f(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int x = t & 63; x < live; x += 64) {
+            const float2 st = a.stat[cell + (int64_t) x * all_rows];
+            sum = fmaf(st.y, __builtin_amdgcn_exp2f(st.x - base), sum);
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+        if ((t & 63) == 0) lse[r] = sum == 0.0f ? INFINITY : base + log2f(sum);
+    }
+    __syncthreads();
+    const float * sco = a.score + head * all_rows * a.score_len;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+        const int j = j0 + u * 256 + t;
+        if (j >= len) return;
+        float add = 0.0f;
+        for (int r = 0; r < rows; ++r) add += __builtin_amdgcn_exp2f(sco[(int64_t) r * a.score_len + j] - lse[r]);
+        a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += add;
+    }
 }
 
 // ---------------------------------------------------------------- eviction
