@@ -168,32 +168,74 @@ static int check_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     return 0;
 }
 
+}  // extern "C"
+
+namespace {
+
 // How a call runs: its kernels, splits and the parts of its workspace (bytes).
 struct AttendPlan {
-    bool few;
-    int split_tiles, n_split, score_len;
-    int64_t part, stat, score, total;
+    bool few, scored, drawn;
+    int rt, row_tiles, split_tiles, n_split, score_len, rows16;
+    int64_t part, stat, score, qh, rowq, total;
 };
 
-static AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
+AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     AttendPlan p{};
     const int64_t len = a->max_len ? a->max_len : c->n_slots, heads = (int64_t) c->n_seq * c->n_kv_head;
     const int64_t group = a->n_head / c->n_kv_head, rows = a->n_rows * group, tiles = (len + 63) / 64;
-    p.few = rows <= (a->weights ? 8 : 32);
-    if (!p.few) {
-        p.total = heads * group * a->n_rows * len * 4;
-        return p;
+    p.few = rows <= 32;
+    p.scored = a->weights && rows <= 8;
+    p.drawn = a->weights && !p.scored;
+    int64_t st;
+    if (p.few) {
+        p.rt = rows <= 16 ? 1 : 2;
+        // 4 tiles (one a wave) to 32 a split, so that there are about 1,024 workgroups: four a CU
+        st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 32) + 3) & ~(int64_t) 3;
+    } else {
+        p.rt = 2;
+        p.row_tiles = (int) ((rows + 64 * p.rt - 1) / (64 * p.rt));
+        // two workgroups a CU, with 8 tiles or more a split
+        const int64_t want = std::max<int64_t>(512 / (heads * p.row_tiles), 1);
+        st = std::max<int64_t>((tiles + want - 1) / want, 8);
     }
-    // 4 tiles (one a wave) to 32 a split, so that there are about 1,024 workgroups: four a CU
-    p.split_tiles = (int) std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 32) + 3 & ~3;
-    p.n_split = (int) ((tiles + p.split_tiles - 1) / p.split_tiles);
-    p.score_len = (int) (tiles * 64);
+    st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
+    p.split_tiles = (int) st;
+    p.n_split = (int) ((tiles + st - 1) / st);
+    p.score_len = (int) std::min<int64_t>(tiles * 64, INT32_MAX);
+    p.rows16 = (int) ((rows + 15) / 16 * 16);
     auto take = [&](int64_t bytes) { const int64_t at = p.total; p.total += (bytes + 255) / 256 * 256; return at; };
     if (p.n_split > 1) p.part = take(heads * p.n_split * rows * c->head_dim * 4);
-    if (p.n_split > 1 || a->weights) p.stat = take(heads * p.n_split * rows * 8);
-    if (a->weights) p.score = take(heads * rows * p.score_len * 4);
+    if (p.n_split > 1 || p.scored) p.stat = take(heads * p.n_split * rows * 8);
+    if (p.scored) p.score = take(heads * rows * p.score_len * 4);
+    if (p.drawn) p.qh = take(heads * p.rows16 * c->head_dim * 2);
+    if (p.drawn) p.rowq = take(heads * p.rows16 * 16);
     return p;
 }
+
+template <int D>
+void launch_attend(const kv8::AttendArgs & a, const AttendPlan & p, hipStream_t st) {
+    const int rows = a.n_rows * a.group, H = a.c.n_kv_head, S = a.c.n_seq;
+    if (p.few) {
+        const dim3 grid(p.n_split, H, S);
+        if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((kv8::k_attend_few<D, 2>), grid, dim3(256), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((kv8::k_attend_tile<D, 2>), dim3(H * S, p.row_tiles, p.n_split), dim3(256), 0, st, a);
+    }
+    if (p.n_split > 8) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), dim3(rows, H, S), dim3(256), 0, st, a);
+    else if (p.n_split > 1)
+        hipLaunchKernelGGL((kv8::k_attend_join<D, false>), dim3((rows + 1024 / D - 1) / (1024 / D), H, S), dim3(256), 0, st, a);
+    if (p.scored) hipLaunchKernelGGL(kv8::k_attend_scored, dim3((a.max_len + 1023) / 1024, H, S), dim3(256), 0, st, a);
+    if (p.drawn) {
+        const int by_rows = rows > 48, tiles = (a.max_len + 63) / 64;
+        hipLaunchKernelGGL(kv8::k_attend_drawn<D>, dim3(by_rows ? tiles : (tiles + 3) / 4, H, S), dim3(256), 0, st, a, by_rows,
+                           p.few ? 8 : 32);
+    }
+}
+
+}  // namespace
+
+extern "C" {
 
 int64_t q3t_kv8_attend_ws(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     t_err[0] = 0;
@@ -211,42 +253,24 @@ int q3t_kv8_attend(int32_t device, const q3t_kv8 * c, const q3t_kv8_attend_args 
     if (plan.total > 0 && (!ws || ws_bytes < plan.total)) return refuse("workspace too small");
     if (!is16(ws)) return refuse("workspace must be 16-byte aligned");
     ON_DEVICE(device);
-    const hipStream_t st = (hipStream_t) stream;
     kv8::AttendArgs a{};
     a.c = *c; a.q = p->q; a.o = p->out;
-    a.qs = p->q_seq; a.qr = p->q_row; a.qh = p->q_head; a.os = p->o_seq; a.orow = p->o_row; a.oh = p->o_head;
+    a.qs = p->q_seq; a.qr = p->q_row; a.qhd = p->q_head; a.os = p->o_seq; a.orow = p->o_row; a.oh = p->o_head;
     a.lens = p->lens; a.n_new = p->n_new; a.len0 = p->len0; a.q_type = p->q_type; a.o_type = p->o_type;
     a.n_rows = p->n_rows; a.n_head = p->n_head; a.group = p->n_head / c->n_kv_head;
     a.max_len = p->max_len ? p->max_len : c->n_slots;
-    a.causal = p->causal != 0; a.weights = p->weights != 0; a.scale = p->scale; a.ws = (float *) ws;
+    a.causal = p->causal != 0; a.weights = p->weights != 0; a.scale = p->scale;
     a.qvec = is16(p->q) && strides16(p->q_type, {p->q_seq, p->q_row, p->q_head});
-    if (plan.few) {
-        a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.score_len = plan.score_len;
-        if (plan.n_split > 1) a.part = (float *) ((char *) ws + plan.part);
-        if (plan.n_split > 1 || a.weights) a.stat = (float2 *) ((char *) ws + plan.stat);
-        if (a.weights) a.score = (float *) ((char *) ws + plan.score);
-        const int rows = a.n_rows * a.group;
-        const dim3 grid(plan.n_split, c->n_kv_head, c->n_seq);
-        if (c->head_dim == 64) {
-            if (rows <= 16) hipLaunchKernelGGL((kv8::k_attend_few<64, 1>), grid, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((kv8::k_attend_few<64, 2>), grid, dim3(256), 0, st, a);
-        } else {
-            if (rows <= 16) hipLaunchKernelGGL((kv8::k_attend_few<128, 1>), grid, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL((kv8::k_attend_few<128, 2>), grid, dim3(256), 0, st, a);
-        }
-        const int blocks = (plan.n_split > 1 ? rows : 0) + (a.weights ? (a.max_len + 1023) / 1024 : 0);
-        if (blocks) {
-            const dim3 jg(blocks, c->n_kv_head, c->n_seq);
-            if (c->head_dim == 64) hipLaunchKernelGGL(kv8::k_attend_join<64>, jg, dim3(256), 0, st, a);
-            else hipLaunchKernelGGL(kv8::k_attend_join<128>, jg, dim3(256), 0, st, a);
-        }
-        return launched("attend");
-    }
-    const dim3 grid(p->n_rows, p->n_head, c->n_seq);
-    if (c->head_dim == 64) hipLaunchKernelGGL(kv8::k_attend_row<64>, grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL(kv8::k_attend_row<128>, grid, dim3(256), 0, st, a);
-    if (a.weights)
-        hipLaunchKernelGGL(kv8::k_attend_acc, dim3((a.max_len + 255) / 256, c->n_kv_head, c->n_seq), dim3(256), 0, st, a);
+    a.ovec = is16(p->out) && strides16(p->o_type, {p->o_seq, p->o_row, p->o_head});
+    a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.dead = !plan.few; a.row_tiles = plan.row_tiles;
+    a.score_len = plan.score_len; a.rows16 = plan.rows16;
+    char * w = (char *) ws;
+    if (plan.n_split > 1) a.part = (float *) (w + plan.part);
+    if (plan.n_split > 1 || plan.scored) a.stat = (float2 *) (w + plan.stat);
+    if (plan.scored) a.score = (float *) (w + plan.score);
+    if (plan.drawn) { a.qh = (uint16_t *) (w + plan.qh); a.rowq = (kv8::f4 *) (w + plan.rowq); }
+    if (c->head_dim == 64) launch_attend<64>(a, plan, (hipStream_t) stream);
+    else launch_attend<128>(a, plan, (hipStream_t) stream);
     return launched("attend");
 }
 

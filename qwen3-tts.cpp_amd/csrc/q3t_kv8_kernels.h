@@ -271,14 +271,17 @@ __global__ __launch_bounds__(2 * D) void k_append(AppendArgs a) {
 struct AttendArgs {
     q3t_kv8 c;
     const void * q; void * o;
-    int64_t qs, qr, qh, os, orow, oh;
+    int64_t qs, qr, qhd, os, orow, oh;
     const int32_t * lens, * n_new;
     int32_t len0, q_type, o_type, n_rows, n_head, group, max_len, causal, weights, qvec, ovec;
     float scale;
-    float * ws;
-    // few rows (k_attend_few, k_attend_join)
-    int32_t split_tiles, n_split, score_len;   // 64-slot tiles a split; scores a row
-    float * part; float2 * stat; float * score; // [seq][kv head][split][row][D], [..][row], [seq][kv head][row][score_len]
+    int32_t split_tiles, n_split;       // 64-slot tiles a split
+    int32_t dead;                       // splits without slots for a row write their sum (0) too
+    int32_t row_tiles;                  // k_attend_tile: row tiles of a sequence and kv head
+    int32_t score_len, rows16;          // scores a row; rows to a multiple of 16
+    // workspace, each where the call needs it: [seq][kv head][split][row][D]; [..][row]: maximum, sum; [seq][kv
+    // head][row][score_len]; [seq][kv head][rows16][D]: q in fp16; [seq][kv head][rows16]: its factor, the row's maximum, 1 / its sum
+    float * part; float2 * stat; float * score; uint16_t * qh; f4 * rowq;
 };
 
 __device__ __forceinline__ int seq_len(const AttendArgs & a, int s) {
@@ -293,92 +296,7 @@ __device__ __forceinline__ int row_limit(const AttendArgs & a, int len, int n, i
     return a.causal ? max(len - n + i + 1, 0) : len;
 }
 
-// One row of one head a workgroup, grid (rows, heads, sequences): its scores to the workspace, their softmax, the
-// value sum by D dims x 256 / D slot groups.  The scores stay as log2 of the
-// probabilities for k_attend_acc.
-template <int D>
-__global__ __launch_bounds__(256) void k_attend_row(AttendArgs a) {
-    __shared__ float q[D], red[8], part[256], top;
-    const int t = threadIdx.x, i = blockIdx.x, h = blockIdx.y, s = blockIdx.z, g = h / a.group;
-    const int len = seq_len(a, s), n = seq_rows(a, s);
-    if (i >= n) return;
-    const int lim = row_limit(a, len, n, i);
-    float * sc = a.ws + (((int64_t) s * a.n_head + h) * a.n_rows + i) * a.max_len;
-    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head, * vb = a.c.v + s * a.c.seq + g * a.c.head;
-    const float * ks = a.c.ks + s * a.c.scale_seq + g * a.c.scale_head, * vs = a.c.vs + s * a.c.scale_seq + g * a.c.scale_head;
-    if (t < D) {
-        const uint16_t x = ((const uint16_t *) a.q)[s * a.qs + i * a.qr + h * a.qh + t];
-        q[t] = a.q_type == kF16 ? h2f(x) : bf2f(x);
-    }
-    __syncthreads();
-    // the row under a power of two that brings its largest value to [1, 2): products with codes stay in range
-    if (t < 64) {
-        float big = 0.0f;
-        for (int d = t; d < D; d += 64) big = fmaxf(big, fabsf(q[d]));
-        big = wave_max_f(big);
-        if (t == 0) top = finite_f(big) && big > 0.0f ? big : 1.0f;
-    }
-    __syncthreads();
-    const int ex = ilogbf(top);
-    if (t < D) q[t] = ldexpf(q[t], -ex);
-    __syncthreads();
-    const float scale = ldexpf(a.scale * 1.4426950408889634f, ex);
-    float m = -INFINITY;
-    for (int j = t; j < lim; j += 256) {
-        float x = 0.0f;
-        const u4 * p = (const u4 *) (kb + (int64_t) j * D);
-        for (int c = 0; c < D / 16; ++c) {
-            const u4 w = p[c];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) x = fmaf((float) byte_of(w[e / 4], e % 4), q[16 * c + e], x);
-        }
-        x *= ks[j / kBlk] * scale;
-        sc[j] = x;
-        m = fmaxf(m, x);
-    }
-    m = wave_max_f(m);
-    if ((t & 63) == 0) red[t >> 6] = m;
-    __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    if (m == -INFINITY) m = 0.0f;
-    float l = 0.0f;
-    for (int j = t; j < lim; j += 256) l += exp2f(sc[j] - m);
-    l = (float) wave_sum_d((double) l);
-    if ((t & 63) == 0) red[4 + (t >> 6)] = l;
-    __syncthreads();
-    l = red[4] + red[5] + red[6] + red[7];
-    const float lse = m + log2f(l);
-    for (int j = t; j < lim; j += 256) sc[j] -= lse;
-    __syncthreads();
-    float o = 0.0f;
-    const int d = t % D;
-    for (int j = t / D; j < lim; j += 256 / D) o = fmaf(exp2f(sc[j]) * vs[j / kBlk], (float) vb[(int64_t) j * D + d], o);
-    part[t] = o;
-    __syncthreads();
-    if (t >= D) return;
-#pragma unroll
-    for (int w = 1; w < 256 / D; ++w) o += part[t + w * D];
-    const int64_t at = s * a.os + i * a.orow + h * a.oh + t;
-    if (a.o_type == kF32) ((float *) a.o)[at] = o;
-    else ((uint16_t *) a.o)[at] = a.o_type == kF16 ? f2h(o) : f2bf(o);
-}
-
-// grid (slots / 256, kv heads, sequences): acc of a slot grows by its
-// probabilities, rows then heads in order.
-__global__ __launch_bounds__(256) void k_attend_acc(AttendArgs a) {
-    const int j = blockIdx.x * 256 + threadIdx.x, g = blockIdx.y, s = blockIdx.z;
-    const int len = seq_len(a, s), n = seq_rows(a, s);
-    if (j >= len || !n) return;
-    float w = 0.0f;
-    for (int i = 0; i < n; ++i) {
-        if (j >= row_limit(a, len, n, i)) continue;
-        for (int e = 0; e < a.group; ++e)
-            w += exp2f(a.ws[(((int64_t) s * a.n_head + g * a.group + e) * a.n_rows + i) * a.max_len + j]);
-    }
-    a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += w;
-}
-
-// ------------------------------------------------ attention of a few rows
+// ----------------------------------------------- operands of attention
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef int i4 __attribute__((ext_vector_type(4)));
@@ -402,19 +320,19 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// One row of q as MFMA operands: lane group k = l / 16 holds dims (D / 4) k + 8 c .. + 7 in q[c], in fp16 under the power
-// of two that brings the row's largest value to [1, 2) (exact for fp16 and for all bits of bfloat16 values down to
-// 2^-14 of the largest).  Returns what a product with it is to be multiplied by, NaN for a row that is not finite.
+// One row of q as MFMA operands: this lane's dims off + step c .. + 7 in q[c], in fp16 under the power of two that
+// brings the row's largest value to [1, 2) (exact for fp16, and for all bits of bfloat16 values down to 2^-14 of the
+// largest), with the sign of the scale.  Returns the factor of a product with it (not negative), NaN for a row that is not finite.
 template <int D>
-__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, h8v (&q)[D / 32]) {
+__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, int off, int step, h8v (&q)[D / 32]) {
     float x[D / 32][8], big = 0.0f, ok = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
         if (on) {
-            if (a.q_type == kF16) load8<kF16>(a.q, at + 8 * c, a.qvec, x[c]);
-            else load8<kBF16>(a.q, at + 8 * c, a.qvec, x[c]);
+            if (a.q_type == kF16) load8<kF16>(a.q, at + off + step * c, a.qvec, x[c]);
+            else load8<kBF16>(a.q, at + off + step * c, a.qvec, x[c]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -430,8 +348,51 @@ __device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, b
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) q[c][e] = (_Float16) ldexpf(x[c][e], -ex);
-    return ldexpf(a.scale * 1.4426950408889634f, ex) + ok;
+        for (int e = 0; e < 8; ++e) {
+            const float y = ldexpf(x[c][e], -ex);
+            q[c][e] = (_Float16) (a.scale < 0.0f ? -y : y);
+        }
+    return ldexpf(fabsf(a.scale) * 1.4426950408889634f, ex) + ok;
+}
+
+// For k_attend_drawn: the row in fp16, and its factor.
+template <int D>
+__device__ __forceinline__ void keep_row(const AttendArgs & a, int64_t head, int row, bool on, bool first, int off, int step,
+                                         const h8v (&q)[D / 32], float qs) {
+    if (!a.qh || !on) return;
+    const int64_t at = head * a.rows16 + row;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) *(h8v *) (a.qh + at * D + off + step * c) = q[c];
+    if (first) a.rowq[at][0] = qs;
+}
+
+template <int N>
+__device__ __forceinline__ void store_out(const AttendArgs & a, int64_t at, const float (&y)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+        if (a.o_type == kF32) {
+            float * p = (float *) a.o + at + j;
+            if (a.ovec) *(f4 *) p = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = y[j + e];
+        } else {
+            uint16_t * p = (uint16_t *) a.o + at + j, h[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[e] = a.o_type == kF16 ? f2h(y[j + e]) : f2bf(y[j + e]);
+            if (a.ovec) *(u2 *) p = (u2){h[0] | (uint32_t) h[1] << 16, h[2] | (uint32_t) h[3] << 16};
+            else
+#pragma unroll
+                for (int e = 0; e < 4; ++e) p[e] = h[e];
+        }
+    }
+}
+
+// The row's maximum and the reciprocal of its sum (0 where it saw no slot).
+__device__ __forceinline__ float inverse(float sum) { return sum == 0.0f ? 0.0f : 1.0f / sum; }
+__device__ __forceinline__ void keep_sum(const AttendArgs & a, int64_t at, float top, float sum) {
+    a.rowq[at][1] = top == -INFINITY ? 0.0f : top;
+    a.rowq[at][2] = inverse(sum);
 }
 
 constexpr float kPScale = 16384.0f;    // probabilities enter the value product times this (fp16's normal range then ends at 2^-28)
@@ -460,7 +421,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + (D / 4) * k, * vb = a.c.v + s * a.c.seq + g * a.c.head + NJ * i;
     const float * sb = (l & 4 ? a.c.vs : a.c.ks) + s * a.c.scale_seq + g * a.c.scale_head;
     const int last = len - 1, last_blk = last / kBlk;
-    float * sco = a.score ? a.score + ((int64_t) s * a.c.n_kv_head + g) * a.n_rows * a.group * a.score_len : nullptr;
+    const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
+    float * sco = a.score ? a.score + hd * a.n_rows * a.group * a.score_len : nullptr;
 
     u4 kr[4][D / 64];
     uint32_t vr[16][NJ / 4];
@@ -505,7 +467,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         const int row = 16 * r + i;
         const bool on = row < rows;
         const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qh + (D / 4) * k, on, q[r]);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, (D / 4) * k, 8, q[r]);
+        if (blockIdx.x == 0 && w == 0) keep_row<D>(a, hd, row, on, k == 0, (D / 4) * k, 8, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
         sum[r] = 0.0f;
@@ -630,77 +593,94 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) all += ml[x][row] * __builtin_amdgcn_exp2f(mm[x][row] - (big == -INFINITY ? 0.0f : big));
         if (at < rows) {
-            const int64_t cell = (((int64_t) s * a.c.n_kv_head + g) * a.n_split + blockIdx.x) * a.n_rows * a.group + at;
+            const int64_t cell = (hd * a.n_split + blockIdx.x) * a.n_rows * a.group + at;
             if (a.stat && d0 == 0) a.stat[cell] = make_float2(big, all);
-            const float inv = a.n_split > 1 ? 1.0f : all == 0.0f ? 0.0f : 1.0f / all;
-            float y[8];
+            if (a.rowq && a.n_split == 1 && d0 == 0) keep_sum(a, hd * a.rows16 + at, big, all);
+            const float inv = a.n_split > 1 ? 1.0f : inverse(all);
+            float y[NJ];
 #pragma unroll
             for (int j = 0; j < NJ; ++j) y[j] = (((mo[0][row][d0 + j] + mo[1][row][d0 + j]) + mo[2][row][d0 + j]) + mo[3][row][d0 + j]) * inv;
             if (a.n_split > 1) {
 #pragma unroll
                 for (int j = 0; j < NJ; j += 4) *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
             } else {
-                const int64_t out = s * a.os + at / a.group * a.orow + (g * a.group + at % a.group) * a.oh + d0;
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    if (a.o_type == kF32) ((float *) a.o)[out + j] = y[j];
-                    else ((uint16_t *) a.o)[out + j] = a.o_type == kF16 ? f2h(y[j]) : f2bf(y[j]);
-                }
+                store_out<NJ>(a, s * a.os + at / a.group * a.orow + (g * a.group + at % a.group) * a.oh + d0, y);
             }
         }
     }
 }
 
-// grid (rows if split, then slots / 1024 if weights are kept; kv heads; sequences).  A row's splits put together: D / 4
-// lanes by 1024 / D groups of splits, the groups added in order; or acc of 1,024 slots from the kept scores.
-template <int D>
+constexpr int kSplitMax = 1024;
+
+// The rows of all splits put together, grid (rows / rows a workgroup, kv heads, sequences): D / 4 lanes a split, many
+// splits of one row (MANY) by 1024 / D groups whose sums are added in order, or a row a group.
+template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     constexpr int LN = D / 4, GR = 256 / LN;
     __shared__ f4 po[GR][LN];
-    __shared__ float pl[GR], lse[8];
-    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    __shared__ float fac[MANY ? kSplitMax : 1], red[8];
+    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z, gr = t / LN, ln = t % LN;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
-    const int live = min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
-    const int64_t head = (int64_t) s * a.c.n_kv_head + g;
-    const int nr = a.n_split > 1 ? all_rows : 0;
-    if ((int) blockIdx.x < nr) {
-        const int row = blockIdx.x, gr = t / LN, ln = t % LN;
-        if (row >= rows) return;
-        const int64_t cell = head * a.n_split * all_rows + row;
-        float top = -INFINITY;
+    const int live = a.dead ? a.n_split : min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
+    const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
+    const int row = MANY ? blockIdx.x : blockIdx.x * GR + gr;
+    if (row >= rows) return;                        // MANY: the whole workgroup
+    const int64_t cell = hd * a.n_split * all_rows + row;
+    float top = -INFINITY, sum = 0.0f;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (MANY) {
+        for (int x = t; x < live; x += 256) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
+        top = wave_max_f(top);
+        if ((t & 63) == 0) red[t >> 6] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int x = t; x < live; x += 256) {
+            const float2 st = a.stat[cell + (int64_t) x * all_rows];
+            fac[x] = __builtin_amdgcn_exp2f(st.x - base);
+            sum = fmaf(st.y, fac[x], sum);
+        }
+#pragma unroll
+        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
+        if ((t & 63) == 0) red[4 + (t >> 6)] = sum;
+        __syncthreads();
+        sum = (red[4] + red[5]) + (red[6] + red[7]);
+#pragma unroll 4
+        for (int x = gr; x < live; x += GR) o += *(const f4 *) (a.part + (cell + (int64_t) x * all_rows) * D + 4 * ln) * fac[x];
+        po[gr][ln] = o;
+        __syncthreads();
+        if (gr) return;
+#pragma unroll
+        for (int x = 1; x < GR; ++x) o += po[x][ln];
+    } else {
         for (int x = 0; x < live; ++x) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
         const float base = top == -INFINITY ? 0.0f : top;
-        f4 o = {0.f, 0.f, 0.f, 0.f};
-        float sum = 0.0f;
-        for (int x = gr; x < live; x += GR) {
+        for (int x = 0; x < live; ++x) {
             const int64_t at = cell + (int64_t) x * all_rows;
             const float2 st = a.stat[at];
+            if (st.y == 0.0f) continue;             // saw no slot: its row is not written
             const float f = __builtin_amdgcn_exp2f(st.x - base);
             o += *(const f4 *) (a.part + at * D + 4 * ln) * f;
             sum = fmaf(st.y, f, sum);
         }
-        po[gr][ln] = o;
-        if (ln == 0) pl[gr] = sum;
-        __syncthreads();
-        if (gr) return;
-#pragma unroll
-        for (int x = 1; x < GR; ++x) {
-            o += po[x][ln];
-            sum += pl[x];
-        }
-        o *= sum == 0.0f ? 0.0f : 1.0f / sum;
-        const int64_t out = s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * ln;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (a.o_type == kF32) ((float *) a.o)[out + e] = o[e];
-            else ((uint16_t *) a.o)[out + e] = a.o_type == kF16 ? f2h(o[e]) : f2bf(o[e]);
-        }
-        return;
     }
-    const int j0 = (blockIdx.x - nr) * 1024;
+    if (a.rowq && ln == 0) keep_sum(a, hd * a.rows16 + row, top, sum);
+    o *= inverse(sum);
+    const float y[4] = {o[0], o[1], o[2], o[3]};
+    store_out<4>(a, s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * ln, y);
+}
+
+// acc of 1,024 slots from the scores that k_attend_few kept, grid (slots / 1024, kv heads, sequences); eight rows at most.
+__global__ __launch_bounds__(256) void k_attend_scored(AttendArgs a) {
+    __shared__ float2 row_sum[8];                   // a row's maximum and the reciprocal of its sum
+    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
+    const int live = min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
+    const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
+    const int j0 = blockIdx.x * 1024;
     if (j0 >= len || !n) return;
-    for (int r = t >> 6; r < rows; r += 4) {        // one wave a row: log2 of the row's sum of exponentials
-        const int64_t cell = head * a.n_split * all_rows + r;
+    for (int r = t >> 6; r < rows; r += 4) {        // one wave a row
+        const int64_t cell = hd * a.n_split * all_rows + r;
         float top = -INFINITY, sum = 0.0f;
         for (int x = t & 63; x < live; x += 64) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
         top = wave_max_f(top);
@@ -711,18 +691,301 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         }
 #pragma unroll
         for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        if ((t & 63) == 0) lse[r] = sum == 0.0f ? INFINITY : base + log2f(sum);
+        if ((t & 63) == 0) row_sum[r] = make_float2(base, inverse(sum));
     }
     __syncthreads();
-    const float * sco = a.score + head * all_rows * a.score_len;
+    const float * sco = a.score + hd * all_rows * a.score_len;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
         const int j = j0 + u * 256 + t;
         if (j >= len) return;
         float add = 0.0f;
-        for (int r = 0; r < rows; ++r) add += __builtin_amdgcn_exp2f(sco[(int64_t) r * a.score_len + j] - lse[r]);
+        for (int r = 0; r < rows; ++r)
+            add = fmaf(__builtin_amdgcn_exp2f(sco[(int64_t) r * a.score_len + j] - row_sum[r].x), row_sum[r].y, add);
         a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += add;
     }
+}
+
+// ----------------------------------------------- attention of many rows
+// A tile of 64 RT rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
+// fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four waves of
+// 16 RT rows.  Tiles of 64 slots become fp16 in LDS once for all rows, double-buffered: the next tile's codes are
+// on their way while this one's products run.  Products, softmax and scales as in k_attend_few; here all
+// waves go through the same tiles, with dims in their own order:
+//   K in LDS: [slot][dim] in 16-byte chunks, chunk c of slot t at c ^ (t % (D / 8));
+//   V in LDS: [dim][8 chunks], chunk 4u + k = slots 32u + 4k + e, then 32u + 16 + 4k + e (an operand of the
+//   value product as it is), at chunk ^ f(dim) with f = (dim / 4) % 8 ^ 2 (dim % 4), so that both the 16 dims of a
+//   read and the 32 dim quads of a write spread over all banks.
+template <int D, int RT>
+__global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
+    constexpr int NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
+    __shared__ __align__(16) uint16_t lds[2][2 * KT];
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
+    const int heads = a.c.n_kv_head, s = blockIdx.x / heads, g = blockIdx.x % heads;
+    const int row_tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, row0 = row_tile * 64 * RT;
+    if (row0 >= rows) return;
+    const int64_t hd = (int64_t) s * heads + g;
+    const int lim_top = row_limit(a, len, n, (min(row0 + 64 * RT, rows) - 1) / a.group);
+    const int t0 = split * a.split_tiles, t1 = min(t0 + a.split_tiles, (lim_top + 63) / 64);
+
+    h8v q[RT][NC];
+    float qs[RT], m[RT], sum[RT], vref = 0.0f;
+    int lim[RT];
+    f4 o[RT][NJ];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = row0 + 16 * (RT * w + r) + i;
+        const bool on = row < rows;
+        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, q[r]);
+        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, q[r], qs[r]);
+        lim[r] = on ? row_limit(a, len, n, tok) : 0;
+        m[r] = -INFINITY;
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
+    }
+    // slots that every row of this wave sees
+    const int lim_all = row_limit(a, len, n, min(row0 + 16 * RT * w, rows - 1) / a.group);
+    // and slots that one of them sees
+    const int lim_one = row0 + 16 * RT * w < rows ? row_limit(a, len, n, (min(row0 + 16 * RT * (w + 1), rows) - 1) / a.group) : 0;
+    const int last = len - 1, last_blk = last / kBlk;
+
+    // staging: 32 bytes of a K row, and 4 dims of 8 V rows a thread; of 64 dims half the threads each
+    const bool do_k = D == 128 || t >= 128, do_v = D == 128 || t < 128;
+    const int kt = D == 128 ? t >> 2 : (t & 127) >> 1, kp = D == 128 ? t & 3 : t & 1;
+    const int vq = t & (D / 4 - 1), vc = (D == 128 ? t : t & 127) / (D / 4);
+    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + 32 * kp, * vb = a.c.v + s * a.c.seq + g * a.c.head + 4 * vq;
+    const float * sb = (l & 4 ? a.c.vs : a.c.ks) + s * a.c.scale_seq + g * a.c.scale_head;
+    u4 kr[2];
+    uint32_t vr[8];
+    float sr = 0.0f;
+    auto fetch = [&](int tile) {
+        if (do_k) {
+            const int8_t * p = kb + (int64_t) min(tile * 64 + kt, last) * D;
+            kr[0] = *(const u4 *) p;
+            kr[1] = *(const u4 *) (p + 16);
+        }
+        if (do_v)
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                vr[e] = *(const uint32_t *) (vb + (int64_t) min(tile * 64 + 32 * (vc >> 2) + 16 * (e >> 2) + 4 * (vc & 3) + (e & 3), last) * D);
+        const int blk = tile * 4 + (l & 3);
+        sr = sb[min(blk, last_blk)];
+        if (blk > last_blk) sr = 0.0f;
+    };
+    auto stash = [&](int buf) {
+        uint16_t * kd = lds[buf], * vd = lds[buf] + KT;
+        if (do_k)
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+                *(h8v *) (kd + kt * D + (((4 * kp + c) ^ (kt & (NCH - 1))) << 3)) = halves8(kr[c / 2][2 * (c & 1)], kr[c / 2][2 * (c & 1) + 1]);
+        if (do_v) {
+            uint32_t f[4][4];
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t w0 = vr[2 * x] ^ 0x80808080u, w1 = vr[2 * x + 1] ^ 0x80808080u;
+                const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+                f[0][x] = halves(lo, kSelLo);
+                f[1][x] = halves(lo, kSelHi);
+                f[2][x] = halves(hi, kSelLo);
+                f[3][x] = halves(hi, kSelHi);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                *(u4 *) (vd + (4 * vq + j) * 64 + ((vc ^ (vq & 7) ^ (2 * j)) << 3)) = (u4){f[j][0], f[j][1], f[j][2], f[j][3]};
+        }
+    };
+    if (t0 < t1) {
+        fetch(t0);
+        stash(0);
+    }
+    float snow = sr;
+    __syncthreads();
+    for (int tile = t0; tile < t1; ++tile) {
+        const uint16_t * kd = lds[(tile - t0) & 1], * vd = kd + KT;
+        if (tile + 1 < t1) fetch(tile + 1);
+        if (tile * 64 < lim_one) {
+            f4 sc[RT][4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) sc[r][b] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const h8v kf = *(const h8v *) (kd + (16 * b + i) * D + (((4 * c + k) ^ (i & (NCH - 1))) << 3));
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf, q[r][c], sc[r][b]);
+                }
+            }
+            float ks[4], vs[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(snow), b));
+                vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(snow), 4 + b));
+            }
+            const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
+            const float vnew = fmaxf(vref, vtop), vscale = vnew > 0.0f ? kPScale / vnew : 0.0f;
+            const float vmove = vnew > vref ? vref / vnew : 1.0f;
+            vref = vnew;
+            h8v p[RT][2];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                // scaled and rounded before the maximum is taken, so that none is above it however large they are
+                float top = -INFINITY;
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    sc[r][b] *= ks[b] * qs[r];
+                    if (tile * 64 + 63 >= lim_all)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            sc[r][b][e] = tile * 64 + 16 * b + 4 * k + e < lim[r] ? sc[r][b][e] : -INFINITY;
+                    top = fmaxf(top, fmaxf(fmaxf(sc[r][b][0], sc[r][b][1]), fmaxf(sc[r][b][2], sc[r][b][3])));
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
+                const float move = __builtin_amdgcn_exp2f(m[r] - base);
+                if (__any(mn > m[r]) || vmove != 1.0f) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) o[r][j] *= move * vmove;
+                }
+                m[r] = mn;
+                float add = 0.0f;
+                uint32_t pw[4][2];
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const float f = vs[b] * vscale;
+                    float x[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
+                        add += x[e];
+                        x[e] *= f;
+                    }
+                    pw[b][0] = pack_h(x[0], x[1]);
+                    pw[b][1] = pack_h(x[2], x[3]);
+                }
+                sum[r] = fmaf(sum[r], move, add);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const i4 v = {(int) pw[2 * u][0], (int) pw[2 * u][1], (int) pw[2 * u + 1][0], (int) pw[2 * u + 1][1]};
+                    p[r][u] = __builtin_bit_cast(h8v, v);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int dim = 16 * j + i;
+                    const h8v vf = *(const h8v *) (vd + dim * 64 + (((4 * u + k) ^ ((dim >> 2) & 7) ^ (2 * (dim & 3))) << 3));
+#pragma unroll
+                    for (int r = 0; r < RT; ++r) o[r][j] = mfma32(vf, p[r][u], o[r][j]);
+                }
+        }
+        if (tile + 1 < t1) stash((tile + 1 - t0) & 1);
+        snow = sr;
+        __syncthreads();
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        sum[r] += __shfl_xor(sum[r], 16);
+        sum[r] += __shfl_xor(sum[r], 32);
+        const int row = row0 + 16 * (RT * w + r) + i;
+        if (row >= rows) continue;
+        const int64_t cell = (hd * a.n_split + split) * a.n_rows * a.group + row;
+        if (a.n_split > 1) {
+            if (k == 0) a.stat[cell] = make_float2(m[r], sum[r]);
+            if (sum[r] == 0.0f) continue;
+        } else if (a.rowq && k == 0) {
+            keep_sum(a, hd * a.rows16 + row, m[r], sum[r]);
+        }
+        const float f = vref / kPScale * (a.n_split > 1 ? 1.0f : inverse(sum[r]));
+        const int64_t out = s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * k;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const f4 x = o[r][j] * f;
+            if (a.n_split > 1) *(f4 *) (a.part + cell * D + 16 * j + 4 * k) = x;
+            else {
+                const float y[4] = {x[0], x[1], x[2], x[3]};
+                store_out<4>(a, out + 16 * j, y);
+            }
+        }
+    }
+}
+
+// acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels left.
+// Scores as there, bit for bit (the same order of dims: `step` 8 of k_attend_few, 32 of k_attend_tile), so that none
+// is above its row's maximum; K in registers; the sum over rows is one over lanes i, in order of the row tiles.
+// by_rows: grid (slot tiles, kv heads, sequences), the four waves take the row tiles in turn and add up; else a wave takes a slot tile.
+template <int D>
+__global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows, int step) {
+    constexpr int NC = D / 32;
+    __shared__ float part[4][64];
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
+    const int heads = a.c.n_kv_head, g = blockIdx.y, s = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
+    const int tile = by_rows ? blockIdx.x : 4 * blockIdx.x + w, j0 = tile * 64;
+    const int64_t hd = (int64_t) s * heads + g;
+    float add[4][4] = {};
+    if (j0 < len && n) {
+        const int last = len - 1, last_blk = last / kBlk;
+        h8v kf[4][NC];
+        float ks[4];
+        const int off = step == 8 ? (D / 4) * k : 8 * k;
+        const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + off;
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int8_t * p = kb + (int64_t) min(j0 + 16 * b + i, last) * D;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const u2 x = *(const u2 *) (p + step * c);
+                kf[b][c] = halves8(x[0], x[1]);
+            }
+            ks[b] = (a.c.ks + s * a.c.scale_seq + g * a.c.scale_head)[min(tile * 4 + b, last_blk)];
+        }
+        // the first row that sees slot j0
+        const int r0 = a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0, rt1 = (rows + 15) / 16;
+        for (int rt = r0 + (by_rows ? w : 0); rt < rt1; rt += by_rows ? 4 : 1) {
+            const int row = 16 * rt + i, rr = min(row, rows - 1);
+            const int64_t at = hd * a.rows16 + rr;
+            const uint16_t * qp = a.qh + at * D + off;
+            const f4 rq = a.rowq[at];
+            h8v q[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (qp + step * c);
+            const int lim = row < rows ? row_limit(a, len, n, rr / a.group) : 0;
+            f4 sc[4];
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                sc[b] = (f4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < NC; ++c) sc[b] = mfma32(kf[b][c], q[c], sc[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < 4; ++b)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = __builtin_amdgcn_exp2f(sc[b][e] * (ks[b] * rq[0]) - rq[1]);
+                    add[b][e] = fmaf(j0 + 16 * b + 4 * k + e < lim ? x : 0.0f, rq[2], add[b][e]);
+                }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < 4; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+#pragma unroll
+            for (int x = 1; x < 16; x <<= 1) add[b][e] += __shfl_xor(add[b][e], x);
+            if (i == 0) part[w][16 * b + 4 * k + e] = add[b][e];
+        }
+    __syncthreads();
+    if (by_rows && w) return;
+    const int j = j0 + l;
+    if (j >= len || !n) return;
+    a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] +=
+        by_rows ? ((part[0][l] + part[1][l]) + part[2][l]) + part[3][l] : part[w][l];
 }
 
 // ---------------------------------------------------------------- eviction
