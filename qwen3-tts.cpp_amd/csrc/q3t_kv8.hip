@@ -189,14 +189,25 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     int64_t st;
     if (p.few) {
         p.rt = rows <= 16 ? 1 : 2;
-        // 4 tiles (one a wave) to 32 a split, so that there are about 1,024 workgroups: four a CU
-        st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 32) + 3) & ~(int64_t) 3;
+        // 4 tiles (one a wave) to 16 a split, so that there are about 1,024 workgroups: four a CU
+        st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 16) + 3) & ~(int64_t) 3;
     } else {
-        p.rt = 2;
-        p.row_tiles = (int) ((rows + 64 * p.rt - 1) / (64 * p.rt));
-        // two workgroups a CU, with 8 tiles or more a split
-        const int64_t want = std::max<int64_t>(512 / (heads * p.row_tiles), 1);
-        st = std::max<int64_t>((tiles + want - 1) / want, 8);
+        p.row_tiles = (int) ((rows + kv8::kTileRows - 1) / kv8::kTileRows);
+        // The shortest splits, of 8 tiles at least, with no more than 600 workgroups, were all sequences as long as the
+        // longest: two a CU run at once, and more would start a third turn.  2,049 rows and slots of 8 x 2 heads, splits
+        // of 8, 9, 10, 12, 17, 33 tiles: 68, 63, 58, 61, 66, 68 us with their joins.
+        const int64_t before = a->causal ? std::max<int64_t>(len - a->n_rows, 0) : len;   // slots that row 0 does not add to
+        auto groups = [&](int64_t of) {
+            int64_t g = 0;
+            for (int64_t r = 0; r < p.row_tiles; ++r) {
+                const int64_t slots = std::min(len, before + (std::min((r + 1) * kv8::kTileRows, rows) + group - 1) / group);
+                g += ((slots + 63) / 64 + of - 1) / of;
+            }
+            return g * heads;
+        };
+        st = 8;
+        while (st < tiles && groups(st) > 600) st += std::max<int64_t>(st / 8, 1);
+        st = std::min(st, std::max<int64_t>(tiles, 1));
     }
     st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
     p.split_tiles = (int) st;
@@ -213,21 +224,22 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
 }
 
 template <int D>
-void launch_attend(const kv8::AttendArgs & a, const AttendPlan & p, hipStream_t st) {
+void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
     const int rows = a.n_rows * a.group, H = a.c.n_kv_head, S = a.c.n_seq;
     if (p.few) {
-        const dim3 grid(p.n_split, H, S);
+        const dim3 grid(H, p.n_split, S);
         if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1>), grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((kv8::k_attend_few<D, 2>), grid, dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((kv8::k_attend_tile<D, 2>), dim3(H * S, p.row_tiles, p.n_split), dim3(256), 0, st, a);
+        hipLaunchKernelGGL((kv8::k_attend_tile<D, 2>), dim3(H * S, p.row_tiles, p.n_split), dim3(kv8::kTileT), 0, st, a);
     }
-    if (p.n_split > 8) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), dim3(rows, H, S), dim3(256), 0, st, a);
-    else if (p.n_split > 1)
-        hipLaunchKernelGGL((kv8::k_attend_join<D, false>), dim3((rows + 1024 / D - 1) / (1024 / D), H, S), dim3(256), 0, st, a);
-    if (p.scored) hipLaunchKernelGGL(kv8::k_attend_scored, dim3((a.max_len + 1023) / 1024, H, S), dim3(256), 0, st, a);
+    const bool many = p.n_split > 8;
+    a.row_blocks = p.n_split == 1 ? 0 : many ? rows : (rows + 1024 / D - 1) / (1024 / D);
+    const dim3 join(a.row_blocks + (p.scored ? (a.max_len + 1023) / 1024 : 0), H, S);
+    if (join.x && many) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), join, dim3(256), 0, st, a);
+    else if (join.x) hipLaunchKernelGGL((kv8::k_attend_join<D, false>), join, dim3(256), 0, st, a);
     if (p.drawn) {
-        const int by_rows = rows > 48, tiles = (a.max_len + 63) / 64;
+        const int tiles = (a.max_len + 63) / 64, by_rows = rows > 48 && (int64_t) (tiles + 3) / 4 * H * S < 512;
         hipLaunchKernelGGL(kv8::k_attend_drawn<D>, dim3(by_rows ? tiles : (tiles + 3) / 4, H, S), dim3(256), 0, st, a, by_rows,
                            p.few ? 8 : 32);
     }
@@ -262,7 +274,7 @@ int q3t_kv8_attend(int32_t device, const q3t_kv8 * c, const q3t_kv8_attend_args 
     a.causal = p->causal != 0; a.weights = p->weights != 0; a.scale = p->scale;
     a.qvec = is16(p->q) && strides16(p->q_type, {p->q_seq, p->q_row, p->q_head});
     a.ovec = is16(p->out) && strides16(p->o_type, {p->o_seq, p->o_row, p->o_head});
-    a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.dead = !plan.few; a.row_tiles = plan.row_tiles;
+    a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.row_tiles = plan.row_tiles;
     a.score_len = plan.score_len; a.rows16 = plan.rows16;
     char * w = (char *) ws;
     if (plan.n_split > 1) a.part = (float *) (w + plan.part);

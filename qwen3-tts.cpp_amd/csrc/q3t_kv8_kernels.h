@@ -276,8 +276,8 @@ struct AttendArgs {
     int32_t len0, q_type, o_type, n_rows, n_head, group, max_len, causal, weights, qvec, ovec;
     float scale;
     int32_t split_tiles, n_split;       // 64-slot tiles a split
-    int32_t dead;                       // splits without slots for a row write their sum (0) too
     int32_t row_tiles;                  // k_attend_tile: row tiles of a sequence and kv head
+    int32_t row_blocks;                 // k_attend_join: workgroups of a sequence and kv head that take rows
     int32_t score_len, rows16;          // scores a row; rows to a multiple of 16
     // workspace, each where the call needs it: [seq][kv head][split][row][D]; [..][row]: maximum, sum; [seq][kv
     // head][row][score_len]; [seq][kv head][rows16][D]: q in fp16; [seq][kv head][rows16]: its factor, the row's maximum, 1 / its sum
@@ -290,6 +290,10 @@ __device__ __forceinline__ int seq_len(const AttendArgs & a, int s) {
 }
 __device__ __forceinline__ int seq_rows(const AttendArgs & a, int s) {
     return a.n_new ? min(max(a.n_new[s], 0), a.n_rows) : a.n_rows;
+}
+// splits that a call's kernels gave `slots` slots: one writes its rows itself, several leave parts for k_attend_join
+__device__ __forceinline__ int splits_of(const AttendArgs & a, int slots) {
+    return ((slots + 63) / 64 + a.split_tiles - 1) / a.split_tiles;
 }
 // slots that row i sees
 __device__ __forceinline__ int row_limit(const AttendArgs & a, int len, int n, int i) {
@@ -320,19 +324,20 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// One row of q as MFMA operands: this lane's dims off + step c .. + 7 in q[c], in fp16 under the power of two that
+// One row of q as MFMA operands: this lane's dims off + lo (c % 2) + hi (c / 2) .. + 7 in q[c], in fp16 under the power of two that
 // brings the row's largest value to [1, 2) (exact for fp16, and for all bits of bfloat16 values down to 2^-14 of the
 // largest), with the sign of the scale.  Returns the factor of a product with it (not negative), NaN for a row that is not finite.
 template <int D>
-__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, int off, int step, h8v (&q)[D / 32]) {
+__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, int off, int lo, int hi,
+                                             h8v (&q)[D / 32]) {
     float x[D / 32][8], big = 0.0f, ok = 0.0f;
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
         if (on) {
-            if (a.q_type == kF16) load8<kF16>(a.q, at + off + step * c, a.qvec, x[c]);
-            else load8<kBF16>(a.q, at + off + step * c, a.qvec, x[c]);
+            if (a.q_type == kF16) load8<kF16>(a.q, at + off + lo * (c & 1) + hi * (c >> 1), a.qvec, x[c]);
+            else load8<kBF16>(a.q, at + off + lo * (c & 1) + hi * (c >> 1), a.qvec, x[c]);
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -357,12 +362,12 @@ __device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, b
 
 // For k_attend_drawn: the row in fp16, and its factor.
 template <int D>
-__device__ __forceinline__ void keep_row(const AttendArgs & a, int64_t head, int row, bool on, bool first, int off, int step,
+__device__ __forceinline__ void keep_row(const AttendArgs & a, int64_t head, int row, bool on, bool first, int off, int lo, int hi,
                                          const h8v (&q)[D / 32], float qs) {
     if (!a.qh || !on) return;
     const int64_t at = head * a.rows16 + row;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) *(h8v *) (a.qh + at * D + off + step * c) = q[c];
+    for (int c = 0; c < D / 32; ++c) *(h8v *) (a.qh + at * D + off + lo * (c & 1) + hi * (c >> 1)) = q[c];
     if (first) a.rowq[at][0] = qs;
 }
 
@@ -395,13 +400,25 @@ __device__ __forceinline__ void keep_sum(const AttendArgs & a, int64_t at, float
     a.rowq[at][2] = inverse(sum);
 }
 
+// The larger of lanes 16 (32) apart, in both, by moves between rows of lanes.
+__device__ __forceinline__ float max_rows(float x) {
+    const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(h[0]), __uint_as_float(h[1]));
+    const auto q = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+
+// A row's base of exponents follows its largest score only once that is more than this above it: a tile then needs
+// no exchange between lanes and no rescaling as a rule, and 2^1.9 kPScale is still an fp16 number.
+constexpr float kSlack = 1.9f;
 constexpr float kPScale = 16384.0f;    // probabilities enter the value product times this (fp16's normal range then ends at 2^-28)
 
-// Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (splits, kv heads, sequences), four
-// waves.  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its own running
+// Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), four
+// waves; workgroups go to the XCDs in turn, so heads come first and a sequence's splits are turned by its number: the
+// first splits, the only ones of short sequences, spread over all XCDs.  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its own running
 // maximum m and sum, and join at the end.
 //   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16,
-//     k = l / 16) holds dims (D / 4) k .. of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
+//     k = l / 16) holds dims 64 c + 16 k .. + 15 of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
 //   - O^T = V^T . P^T: those probabilities are the B operand where they lie, if the 32 slots of an MFMA
 //     are taken as 4k + e of one block of 16, then of the next; lane (i, k) then needs the codes of dims (D / 16) i .. of
 //     those slots, which it reads as one piece of a row, and turns round by byte permutations while they
@@ -414,11 +431,12 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
     __shared__ float mo[4][16][LD], mm[4][16], ml[4][16];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
-    const int g = blockIdx.y, s = blockIdx.z;
+    const int g = blockIdx.x, s = blockIdx.z, split = (blockIdx.y + s) % a.n_split;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
-    const int tiles = (len + 63) / 64, t0 = blockIdx.x * a.split_tiles, t1 = min(t0 + a.split_tiles, tiles);
-    if (!n || (blockIdx.x && t0 >= tiles)) return;
-    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + (D / 4) * k, * vb = a.c.v + s * a.c.seq + g * a.c.head + NJ * i;
+    const int tiles = (len + 63) / 64, t0 = split * a.split_tiles, t1 = min(t0 + a.split_tiles, tiles);
+    if (!n || (split && t0 >= tiles)) return;
+    const bool parts = splits_of(a, len) > 1;
+    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head, * vb = a.c.v + s * a.c.seq + g * a.c.head;
     const float * sb = (l & 4 ? a.c.vs : a.c.ks) + s * a.c.scale_seq + g * a.c.scale_head;
     const int last = len - 1, last_blk = last / kBlk;
     const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
@@ -427,31 +445,32 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     u4 kr[4][D / 64];
     uint32_t vr[16][NJ / 4];
     float sr;
+    // rows past the last slot are the last slot's again; a scale past it is taken as 0 where it is used (a choice here
+    // would wait for the load)
     auto fetch_k = [&](int tile) {
-#pragma unroll
-        for (int b = 0; b < 4; ++b) {
-            const int8_t * p = kb + (int64_t) min(tile * 64 + 16 * b + i, last) * D;
-#pragma unroll
-            for (int c = 0; c < D / 64; ++c) kr[b][c] = *(const u4 *) (p + 16 * c);
-        }
-        const int blk = tile * 4 + (l & 3);
-        sr = sb[min(blk, last_blk)];
-        if (blk > last_blk) sr = 0.0f;
-    };
-    auto fetch_v = [&](int tile) {
+        const int8_t * p = kb + (int64_t) tile * 64 * D;
+        const int left = last - tile * 64;
 #pragma unroll
         for (int b = 0; b < 4; ++b)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int8_t * p = vb + (int64_t) min(tile * 64 + 16 * b + 4 * k + e, last) * D;
-                if constexpr (D == 128) {
-                    const u2 x = *(const u2 *) p;
-                    vr[4 * b + e][0] = x[0];
-                    vr[4 * b + e][1] = x[1];
-                } else {
-                    vr[4 * b + e][0] = *(const uint32_t *) p;
-                }
+            for (int c = 0; c < D / 64; ++c)
+                kr[b][c] = *(const u4 *) (p + (uint32_t) (min(16 * b + i, left) * D + 64 * c + 16 * k));
+        sr = sb[min(tile * 4 + (l & 3), last_blk)];
+    };
+    auto fetch_v = [&](int tile) {
+        const int8_t * p = vb + (int64_t) tile * 64 * D;
+        const int left = last - tile * 64;
+#pragma unroll
+        for (int x = 0; x < 16; ++x) {
+            const uint32_t off = (uint32_t) (min(16 * (x / 4) + 4 * k + x % 4, left) * D + NJ * i);
+            if constexpr (D == 128) {
+                const u2 y = *(const u2 *) (p + off);
+                vr[x][0] = y[0];
+                vr[x][1] = y[1];
+            } else {
+                vr[x][0] = *(const uint32_t *) (p + off);
             }
+        }
     };
     const int first = t0 + w;
     if (first < t1) {
@@ -459,7 +478,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         fetch_v(first);
     }
     h8v q[RT][NC];
-    float qs[RT], m[RT], sum[RT], vref = 0.0f;
+    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
     int lim[RT];
     f4 o[RT][NJ];
 #pragma unroll
@@ -467,8 +486,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         const int row = 16 * r + i;
         const bool on = row < rows;
         const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, (D / 4) * k, 8, q[r]);
-        if (blockIdx.x == 0 && w == 0) keep_row<D>(a, hd, row, on, k == 0, (D / 4) * k, 8, q[r], qs[r]);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 16 * k, 8, 64, q[r]);
+        if (split == 0 && w == 0) keep_row<D>(a, hd, row, on, k == 0, 16 * k, 8, 64, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
         sum[r] = 0.0f;
@@ -489,17 +508,21 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
                 for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf, q[r][c], sc[r][b]);
             }
         }
+        const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
         float ks[4], vs[4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
-            ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sr), b));
-            vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(sr), 4 + b));
+            ks[b] = __int_as_float(__builtin_amdgcn_readlane(sl, b));
+            vs[b] = __int_as_float(__builtin_amdgcn_readlane(sl, 4 + b));
         }
         if (tile + 4 < t1) fetch_k(tile + 4);
         const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-        const float vnew = fmaxf(vref, vtop), vscale = vnew > 0.0f ? kPScale / vnew : 0.0f;
-        const float vmove = vnew > vref ? vref / vnew : 1.0f;
-        vref = vnew;
+        float vmove = 1.0f;
+        if (vtop > vref) {
+            vmove = vref / vtop;
+            vref = vtop;
+            vscale = kPScale / vref;
+        }
         h8v p[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -518,30 +541,30 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
                     *(f4 *) (sco + (int64_t) (16 * r + i) * a.score_len + tile * 64 + 16 * b + 4 * k) = sc[r][b];
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
-            const float move = __builtin_amdgcn_exp2f(m[r] - base);     // 0 at first
-            if (__any(mn > m[r]) || vmove != 1.0f) {
+            if (__any(top > m[r] + kSlack)) {
+                const float mn = fmaxf(m[r], max_rows(top)), move = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - mn);
+                m[r] = mn;
+                sum[r] *= move;
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) o[r][j] *= move * vmove;
+                for (int j = 0; j < NJ; ++j) o[r][j] *= move;
             }
-            m[r] = mn;
-            float add = 0.0f;
+            if (vmove != 1.0f)
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) o[r][j] *= vmove;
+            const float base = m[r] == -INFINITY ? 0.0f : m[r];
+            float add[4];
             uint32_t pw[4][2];
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
+                const float f = vs[b] * vscale;
                 float x[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
-                    add += x[e];
-                    x[e] *= vs[b] * vscale;
-                }
-                pw[b][0] = pack_h(x[0], x[1]);
-                pw[b][1] = pack_h(x[2], x[3]);
+                for (int e = 0; e < 4; ++e) x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
+                add[b] = (x[0] + x[1]) + (x[2] + x[3]);
+                pw[b][0] = pack_h(x[0] * f, x[1] * f);
+                pw[b][1] = pack_h(x[2] * f, x[3] * f);
             }
-            sum[r] = fmaf(sum[r], move, add);
+            sum[r] += (add[0] + add[1]) + (add[2] + add[3]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const i4 v = {(int) pw[2 * u][0], (int) pw[2 * u][1], (int) pw[2 * u + 1][0], (int) pw[2 * u + 1][1]};
@@ -593,14 +616,14 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int x = 0; x < 4; ++x) all += ml[x][row] * __builtin_amdgcn_exp2f(mm[x][row] - (big == -INFINITY ? 0.0f : big));
         if (at < rows) {
-            const int64_t cell = (hd * a.n_split + blockIdx.x) * a.n_rows * a.group + at;
+            const int64_t cell = (hd * a.n_split + split) * a.n_rows * a.group + at;
             if (a.stat && d0 == 0) a.stat[cell] = make_float2(big, all);
-            if (a.rowq && a.n_split == 1 && d0 == 0) keep_sum(a, hd * a.rows16 + at, big, all);
-            const float inv = a.n_split > 1 ? 1.0f : inverse(all);
+            if (a.rowq && !parts && d0 == 0) keep_sum(a, hd * a.rows16 + at, big, all);
+            const float inv = parts ? 1.0f : inverse(all);
             float y[NJ];
 #pragma unroll
             for (int j = 0; j < NJ; ++j) y[j] = (((mo[0][row][d0 + j] + mo[1][row][d0 + j]) + mo[2][row][d0 + j]) + mo[3][row][d0 + j]) * inv;
-            if (a.n_split > 1) {
+            if (parts) {
 #pragma unroll
                 for (int j = 0; j < NJ; j += 4) *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
             } else {
@@ -611,20 +634,68 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 }
 
 constexpr int kSplitMax = 1024;
+constexpr int kTileT = 256, kTileRows = 128;
 
-// The rows of all splits put together, grid (rows / rows a workgroup, kv heads, sequences): D / 4 lanes a split, many
+// acc of 1,024 slots (the blk-th) from the scores that k_attend_few kept; eight rows at most.
+__device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
+    __shared__ float2 row_sum[8];                   // a row's maximum and the reciprocal of its sum
+    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
+    const int live = splits_of(a, len);
+    const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
+    const int j = blk * 1024 + 4 * t;               // this thread's four slots
+    if (blk * 1024 >= len || !n) return;
+    const float * sco = a.score + hd * all_rows * a.score_len + min(j, a.score_len - 4);
+    float * acc = a.c.acc + s * a.c.acc_seq + g * a.c.acc_head + j;
+    f4 x[8], old = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        if (r < rows) x[r] = *(const f4 *) (sco + (int64_t) r * a.score_len);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < len) old[e] = acc[e];
+    for (int r = t >> 6; r < rows; r += 4) {        // one wave a row
+        const int64_t cell = hd * a.n_split * all_rows + r;
+        float top = -INFINITY, sum = 0.0f;
+        for (int y = t & 63; y < live; y += 64) top = fmaxf(top, a.stat[cell + (int64_t) y * all_rows].x);
+        top = wave_max_f(top);
+        const float base = top == -INFINITY ? 0.0f : top;
+        for (int y = t & 63; y < live; y += 64) {
+            const float2 st = a.stat[cell + (int64_t) y * all_rows];
+            sum = fmaf(st.y, __builtin_amdgcn_exp2f(st.x - base), sum);
+        }
+#pragma unroll
+        for (int y = 1; y < 64; y <<= 1) sum += __shfl_xor(sum, y);
+        if ((t & 63) == 0) row_sum[r] = make_float2(base, inverse(sum));
+    }
+    __syncthreads();
+    f4 add = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int r = 0; r < 8; ++r)
+        if (r < rows)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) add[e] = fmaf(__builtin_amdgcn_exp2f(x[r][e] - row_sum[r].x), row_sum[r].y, add[e]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (j + e < len) acc[e] = old[e] + add[e];
+}
+
+// The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores were
+// kept; kv heads; sequences): D / 4 lanes a split, many
 // splits of one row (MANY) by 1024 / D groups whose sums are added in order, or a row a group.
 template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     constexpr int LN = D / 4, GR = 256 / LN;
     __shared__ f4 po[GR][LN];
     __shared__ float fac[MANY ? kSplitMax : 1], red[8];
+    if ((int) blockIdx.x >= a.row_blocks) return scored_slots(a, blockIdx.x - a.row_blocks);
     const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z, gr = t / LN, ln = t % LN;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
-    const int live = a.dead ? a.n_split : min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
     const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
     const int row = MANY ? blockIdx.x : blockIdx.x * GR + gr;
     if (row >= rows) return;                        // MANY: the whole workgroup
+    const int live = splits_of(a, a.row_tiles ? row_limit(a, len, n, (min((row / kTileRows + 1) * kTileRows, rows) - 1) / a.group) : len);
+    if (live <= 1) return;                          // written by its split
     const int64_t cell = hd * a.n_split * all_rows + row;
     float top = -INFINITY, sum = 0.0f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
@@ -670,56 +741,22 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     store_out<4>(a, s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * ln, y);
 }
 
-// acc of 1,024 slots from the scores that k_attend_few kept, grid (slots / 1024, kv heads, sequences); eight rows at most.
-__global__ __launch_bounds__(256) void k_attend_scored(AttendArgs a) {
-    __shared__ float2 row_sum[8];                   // a row's maximum and the reciprocal of its sum
-    const int t = threadIdx.x, g = blockIdx.y, s = blockIdx.z;
-    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, all_rows = a.n_rows * a.group;
-    const int live = min((len + 64 * a.split_tiles - 1) / (64 * a.split_tiles), a.n_split);
-    const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
-    const int j0 = blockIdx.x * 1024;
-    if (j0 >= len || !n) return;
-    for (int r = t >> 6; r < rows; r += 4) {        // one wave a row
-        const int64_t cell = hd * a.n_split * all_rows + r;
-        float top = -INFINITY, sum = 0.0f;
-        for (int x = t & 63; x < live; x += 64) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
-        top = wave_max_f(top);
-        const float base = top == -INFINITY ? 0.0f : top;
-        for (int x = t & 63; x < live; x += 64) {
-            const float2 st = a.stat[cell + (int64_t) x * all_rows];
-            sum = fmaf(st.y, __builtin_amdgcn_exp2f(st.x - base), sum);
-        }
-#pragma unroll
-        for (int x = 1; x < 64; x <<= 1) sum += __shfl_xor(sum, x);
-        if ((t & 63) == 0) row_sum[r] = make_float2(base, inverse(sum));
-    }
-    __syncthreads();
-    const float * sco = a.score + hd * all_rows * a.score_len;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const int j = j0 + u * 256 + t;
-        if (j >= len) return;
-        float add = 0.0f;
-        for (int r = 0; r < rows; ++r)
-            add = fmaf(__builtin_amdgcn_exp2f(sco[(int64_t) r * a.score_len + j] - row_sum[r].x), row_sum[r].y, add);
-        a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += add;
-    }
-}
-
 // ----------------------------------------------- attention of many rows
 // A tile of 64 RT rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
 // fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four waves of
-// 16 RT rows.  Tiles of 64 slots become fp16 in LDS once for all rows, double-buffered: the next tile's codes are
-// on their way while this one's products run.  Products, softmax and scales as in k_attend_few; here all
-// waves go through the same tiles, with dims in their own order:
+// 16 RT rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
+// k_attend_few; here all waves go through the same tiles, with dims in their own order:
 //   K in LDS: [slot][dim] in 16-byte chunks, chunk c of slot t at c ^ (t % (D / 8));
 //   V in LDS: [dim][8 chunks], chunk 4u + k = slots 32u + 4k + e, then 32u + 16 + 4k + e (an operand of the
 //   value product as it is), at chunk ^ f(dim) with f = (dim / 4) % 8 ^ 2 (dim % 4), so that both the 16 dims of a
 //   read and the 32 dim quads of a write spread over all banks.
+// Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to LDS
+// at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the MFMAs of
+// these: left to itself the compiler waits for each read alone.
 template <int D, int RT>
-__global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
+__global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
-    __shared__ __align__(16) uint16_t lds[2][2 * KT];
+    __shared__ __align__(16) uint16_t lds[4 * KT];      // K of even and odd tiles, V of even and odd tiles
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
     const int heads = a.c.n_kv_head, s = blockIdx.x / heads, g = blockIdx.x % heads;
     const int row_tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
@@ -728,9 +765,12 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
     const int64_t hd = (int64_t) s * heads + g;
     const int lim_top = row_limit(a, len, n, (min(row0 + 64 * RT, rows) - 1) / a.group);
     const int t0 = split * a.split_tiles, t1 = min(t0 + a.split_tiles, (lim_top + 63) / 64);
+    const bool parts = splits_of(a, lim_top) > 1;
+    if (split && t0 >= t1) return;
+    const bool work = row0 + 16 * RT * w < rows;        // this wave has rows
 
     h8v q[RT][NC];
-    float qs[RT], m[RT], sum[RT], vref = 0.0f;
+    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
     int lim[RT];
     f4 o[RT][NJ];
 #pragma unroll
@@ -738,136 +778,160 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
         const int row = row0 + 16 * (RT * w + r) + i;
         const bool on = row < rows;
         const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, q[r]);
-        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, q[r], qs[r]);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, 64, q[r]);
+        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, 64, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
         sum[r] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
-    // slots that every row of this wave sees
-    const int lim_all = row_limit(a, len, n, min(row0 + 16 * RT * w, rows - 1) / a.group);
-    // and slots that one of them sees
-    const int lim_one = row0 + 16 * RT * w < rows ? row_limit(a, len, n, (min(row0 + 16 * RT * (w + 1), rows) - 1) / a.group) : 0;
+    const int plain = row_limit(a, len, n, row0 / a.group) / 64;    // tiles before this one need no mask
     const int last = len - 1, last_blk = last / kBlk;
 
     // staging: 32 bytes of a K row, and 4 dims of 8 V rows a thread; of 64 dims half the threads each
     const bool do_k = D == 128 || t >= 128, do_v = D == 128 || t < 128;
     const int kt = D == 128 ? t >> 2 : (t & 127) >> 1, kp = D == 128 ? t & 3 : t & 1;
     const int vq = t & (D / 4 - 1), vc = (D == 128 ? t : t & 127) / (D / 4);
-    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + 32 * kp, * vb = a.c.v + s * a.c.seq + g * a.c.head + 4 * vq;
+    const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head, * vb = a.c.v + s * a.c.seq + g * a.c.head;
     const float * sb = (l & 4 ? a.c.vs : a.c.ks) + s * a.c.scale_seq + g * a.c.scale_head;
     u4 kr[2];
     uint32_t vr[8];
     float sr = 0.0f;
-    auto fetch = [&](int tile) {
-        if (do_k) {
-            const int8_t * p = kb + (int64_t) min(tile * 64 + kt, last) * D;
-            kr[0] = *(const u4 *) p;
-            kr[1] = *(const u4 *) (p + 16);
-        }
-        if (do_v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-                vr[e] = *(const uint32_t *) (vb + (int64_t) min(tile * 64 + 32 * (vc >> 2) + 16 * (e >> 2) + 4 * (vc & 3) + (e & 3), last) * D);
-        const int blk = tile * 4 + (l & 3);
-        sr = sb[min(blk, last_blk)];
-        if (blk > last_blk) sr = 0.0f;
+    // tiles past the split's end are its last one again, rows past the last slot the last slot's
+    auto fetch_k = [&](int tile) {
+        if (!do_k) return;
+        tile = min(tile, t1 - 1);
+        const int8_t * p = kb + (int64_t) tile * 64 * D;
+        const uint32_t off = (uint32_t) (min(kt, last - tile * 64) * D + 32 * kp);
+        kr[0] = *(const u4 *) (p + off);
+        kr[1] = *(const u4 *) (p + off + 16);
     };
-    auto stash = [&](int buf) {
-        uint16_t * kd = lds[buf], * vd = lds[buf] + KT;
-        if (do_k)
+    auto fetch_v = [&](int tile) {
+        tile = min(tile, t1 - 1);
+        sr = sb[min(tile * 4 + (l & 3), last_blk)];
+        if (!do_v) return;
+        const int8_t * p = vb + (int64_t) tile * 64 * D;
+        const int left = last - tile * 64;
 #pragma unroll
-            for (int c = 0; c < 4; ++c)
-                *(h8v *) (kd + kt * D + (((4 * kp + c) ^ (kt & (NCH - 1))) << 3)) = halves8(kr[c / 2][2 * (c & 1)], kr[c / 2][2 * (c & 1) + 1]);
-        if (do_v) {
-            uint32_t f[4][4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const uint32_t w0 = vr[2 * x] ^ 0x80808080u, w1 = vr[2 * x + 1] ^ 0x80808080u;
-                const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
-                f[0][x] = halves(lo, kSelLo);
-                f[1][x] = halves(lo, kSelHi);
-                f[2][x] = halves(hi, kSelLo);
-                f[3][x] = halves(hi, kSelHi);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                *(u4 *) (vd + (4 * vq + j) * 64 + ((vc ^ (vq & 7) ^ (2 * j)) << 3)) = (u4){f[j][0], f[j][1], f[j][2], f[j][3]};
-        }
+        for (int e = 0; e < 8; ++e)
+            vr[e] = *(const uint32_t *) (p + (uint32_t) (min(32 * (vc >> 2) + 16 * (e >> 2) + 4 * (vc & 3) + (e & 3), left) * D + 4 * vq));
     };
-    if (t0 < t1) {
-        fetch(t0);
-        stash(0);
-    }
-    float snow = sr;
-    __syncthreads();
-    for (int tile = t0; tile < t1; ++tile) {
-        const uint16_t * kd = lds[(tile - t0) & 1], * vd = kd + KT;
-        if (tile + 1 < t1) fetch(tile + 1);
-        if (tile * 64 < lim_one) {
+    auto stash_k = [&](int tile) {
+        if (!do_k) return;
+        uint16_t * d = lds + (tile & 1) * KT + kt * D;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            *(h8v *) (d + (((4 * kp + c) ^ (kt & (NCH - 1))) << 3)) = halves8(kr[c / 2][2 * (c & 1)], kr[c / 2][2 * (c & 1) + 1]);
+    };
+    auto stash_v = [&](int tile) {
+        if (!do_v) return;
+        uint16_t * d = lds + (2 + (tile & 1)) * KT + 4 * vq * 64;
+        uint32_t f[4][4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t w0 = vr[2 * x] ^ 0x80808080u, w1 = vr[2 * x + 1] ^ 0x80808080u;
+            const uint32_t lo = __builtin_amdgcn_perm(w1, w0, 0x05010400u), hi = __builtin_amdgcn_perm(w1, w0, 0x07030602u);
+            f[0][x] = halves(lo, kSelLo);
+            f[1][x] = halves(lo, kSelHi);
+            f[2][x] = halves(hi, kSelLo);
+            f[3][x] = halves(hi, kSelHi);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            *(u4 *) (d + j * 64 + ((vc ^ (vq & 7) ^ (2 * j)) << 3)) = (u4){f[j][0], f[j][1], f[j][2], f[j][3]};
+    };
+    auto step = [&](int tile, auto masked) {
+        const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
+        fetch_k(tile + 1);
+        fetch_v(tile + 1);
+        float ks[4], vs[4];
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            ks[b] = __int_as_float(__builtin_amdgcn_readlane(sl, b));
+            vs[b] = __int_as_float(__builtin_amdgcn_readlane(sl, 4 + b));
+        }
+        if (work) {
+            const uint16_t * kd = lds + (tile & 1) * KT + i * D, * vd = lds + (2 + (tile & 1)) * KT + i * 64;
             f4 sc[RT][4];
+            h8v kf[2][4];
+            auto read_k = [&](int c) {
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
+                for (int b = 0; b < 4; ++b)
+                    kf[c & 1][b] = *(const h8v *) (kd + 16 * b * D + (((4 * c + k) ^ (i & (NCH - 1))) << 3));
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            read_k(0);
 #pragma unroll
-                for (int r = 0; r < RT; ++r) sc[r][b] = (f4){0.f, 0.f, 0.f, 0.f};
+            for (int c = 0; c < NC; ++c) {
+                if (c + 1 < NC) read_k(c + 1);
 #pragma unroll
-                for (int c = 0; c < NC; ++c) {
-                    const h8v kf = *(const h8v *) (kd + (16 * b + i) * D + (((4 * c + k) ^ (i & (NCH - 1))) << 3));
+                for (int b = 0; b < 4; ++b)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf, q[r][c], sc[r][b]);
-                }
-            }
-            float ks[4], vs[4];
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                ks[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(snow), b));
-                vs[b] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(snow), 4 + b));
+                    for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf[c & 1][b], q[r][c], c ? sc[r][b] : (f4){0.f, 0.f, 0.f, 0.f});
             }
             const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            const float vnew = fmaxf(vref, vtop), vscale = vnew > 0.0f ? kPScale / vnew : 0.0f;
-            const float vmove = vnew > vref ? vref / vnew : 1.0f;
-            vref = vnew;
-            h8v p[RT][2];
+            float vmove = 1.0f;
+            if (vtop > vref) {
+                vmove = vref / vtop;
+                vref = vtop;
+                vscale = kPScale / vref;
+            }
+            bool grows = vmove != 1.0f;
+            float top[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
                 // scaled and rounded before the maximum is taken, so that none is above it however large they are
-                float top = -INFINITY;
+                top[r] = -INFINITY;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     sc[r][b] *= ks[b] * qs[r];
-                    if (tile * 64 + 63 >= lim_all)
+                    if constexpr (decltype(masked)::value)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             sc[r][b][e] = tile * 64 + 16 * b + 4 * k + e < lim[r] ? sc[r][b][e] : -INFINITY;
-                    top = fmaxf(top, fmaxf(fmaxf(sc[r][b][0], sc[r][b][1]), fmaxf(sc[r][b][2], sc[r][b][3])));
+                    top[r] = fmaxf(top[r], fmaxf(fmaxf(sc[r][b][0], sc[r][b][1]), fmaxf(sc[r][b][2], sc[r][b][3])));
                 }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float mn = fmaxf(m[r], top), base = mn == -INFINITY ? 0.0f : mn;
-                const float move = __builtin_amdgcn_exp2f(m[r] - base);
-                if (__any(mn > m[r]) || vmove != 1.0f) {
+                grows |= top[r] > m[r] + kSlack;
+            }
+            if (__any(grows)) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) {
+                    const float mn = fmaxf(m[r], max_rows(top[r]));
+                    const float move = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[r] - mn);
+                    m[r] = mn;
+                    sum[r] *= move;
 #pragma unroll
                     for (int j = 0; j < NJ; ++j) o[r][j] *= move * vmove;
                 }
-                m[r] = mn;
-                float add = 0.0f;
+            }
+            // chunk 4u + k of dim 16 j + i: at (4 (u ^ j % 2) + k) ^ (i / 4) ^ 2 (i % 4)
+            const int x0 = (k ^ (i >> 2) ^ (2 * (i & 3))) << 3;
+            h8v vf[2][4];                           // of two dim tiles: u 0 of both, u 1 of both
+            auto read_v = [&](int j) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    vf[(j / 2) & 1][x] = *(const h8v *) (vd + 16 * (j + (x & 1)) * 64 + (x0 ^ (32 * ((x >> 1) ^ (x & 1)))));
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            read_v(0);
+            h8v p[RT][2];
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const float base = m[r] == -INFINITY ? 0.0f : m[r];
                 uint32_t pw[4][2];
+                float add = 0.0f;
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const float f = vs[b] * vscale;
                     float x[4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
-                        add += x[e];
-                        x[e] *= f;
-                    }
-                    pw[b][0] = pack_h(x[0], x[1]);
-                    pw[b][1] = pack_h(x[2], x[3]);
+                    for (int e = 0; e < 4; ++e) x[e] = __builtin_amdgcn_exp2f(sc[r][b][e] - base);
+                    add += (x[0] + x[1]) + (x[2] + x[3]);
+                    pw[b][0] = pack_h(x[0] * f, x[1] * f);
+                    pw[b][1] = pack_h(x[2] * f, x[3] * f);
                 }
-                sum[r] = fmaf(sum[r], move, add);
+                sum[r] += add;
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const i4 v = {(int) pw[2 * u][0], (int) pw[2 * u][1], (int) pw[2 * u + 1][0], (int) pw[2 * u + 1][1]};
@@ -875,18 +939,27 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
                 }
             }
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NJ; j += 2) {
+                if (j + 2 < NJ) read_v(j + 2);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int dim = 16 * j + i;
-                    const h8v vf = *(const h8v *) (vd + dim * 64 + (((4 * u + k) ^ ((dim >> 2) & 7) ^ (2 * (dim & 3))) << 3));
+                for (int x = 0; x < 4; ++x)
 #pragma unroll
-                    for (int r = 0; r < RT; ++r) o[r][j] = mfma32(vf, p[r][u], o[r][j]);
-                }
+                    for (int r = 0; r < RT; ++r) o[r][j + (x & 1)] = mfma32(vf[(j / 2) & 1][x], p[r][x >> 1], o[r][j + (x & 1)]);
+            }
         }
-        if (tile + 1 < t1) stash((tile + 1 - t0) & 1);
-        snow = sr;
+        stash_k(tile + 1);
+        stash_v(tile + 1);
         __syncthreads();
+    };
+    if (t0 < t1) {
+        fetch_k(t0);
+        fetch_v(t0);
+        stash_k(t0);
+        stash_v(t0);
+        __syncthreads();
+        int tile = t0;
+        for (; tile < min(t1, plain); ++tile) step(tile, std::false_type{});
+        for (; tile < t1; ++tile) step(tile, std::true_type{});
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -895,18 +968,18 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
         const int row = row0 + 16 * (RT * w + r) + i;
         if (row >= rows) continue;
         const int64_t cell = (hd * a.n_split + split) * a.n_rows * a.group + row;
-        if (a.n_split > 1) {
+        if (parts) {
             if (k == 0) a.stat[cell] = make_float2(m[r], sum[r]);
             if (sum[r] == 0.0f) continue;
         } else if (a.rowq && k == 0) {
             keep_sum(a, hd * a.rows16 + row, m[r], sum[r]);
         }
-        const float f = vref / kPScale * (a.n_split > 1 ? 1.0f : inverse(sum[r]));
+        const float f = vref / kPScale * (parts ? 1.0f : inverse(sum[r]));
         const int64_t out = s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * k;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const f4 x = o[r][j] * f;
-            if (a.n_split > 1) *(f4 *) (a.part + cell * D + 16 * j + 4 * k) = x;
+            if (parts) *(f4 *) (a.part + cell * D + 16 * j + 4 * k) = x;
             else {
                 const float y[4] = {x[0], x[1], x[2], x[3]};
                 store_out<4>(a, out + 16 * j, y);
@@ -916,11 +989,11 @@ __global__ __launch_bounds__(256) void k_attend_tile(AttendArgs a) {
 }
 
 // acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels left.
-// Scores as there, bit for bit (the same order of dims: `step` 8 of k_attend_few, 32 of k_attend_tile), so that none
+// Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that none
 // is above its row's maximum; K in registers; the sum over rows is one over lanes i, in order of the row tiles.
 // by_rows: grid (slot tiles, kv heads, sequences), the four waves take the row tiles in turn and add up; else a wave takes a slot tile.
 template <int D>
-__global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows, int step) {
+__global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows, int lo) {
     constexpr int NC = D / 32;
     __shared__ float part[4][64];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
@@ -933,43 +1006,52 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows,
         const int last = len - 1, last_blk = last / kBlk;
         h8v kf[4][NC];
         float ks[4];
-        const int off = step == 8 ? (D / 4) * k : 8 * k;
+        const int off = lo == 8 ? 16 * k : 8 * k;
         const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + off;
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
             const int8_t * p = kb + (int64_t) min(j0 + 16 * b + i, last) * D;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                const u2 x = *(const u2 *) (p + step * c);
+                const u2 x = *(const u2 *) (p + lo * (c & 1) + 64 * (c >> 1));
                 kf[b][c] = halves8(x[0], x[1]);
             }
             ks[b] = (a.c.ks + s * a.c.scale_seq + g * a.c.scale_head)[min(tile * 4 + b, last_blk)];
         }
         // the first row that sees slot j0
-        const int r0 = a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0, rt1 = (rows + 15) / 16;
-        for (int rt = r0 + (by_rows ? w : 0); rt < rt1; rt += by_rows ? 4 : 1) {
-            const int row = 16 * rt + i, rr = min(row, rows - 1);
-            const int64_t at = hd * a.rows16 + rr;
-            const uint16_t * qp = a.qh + at * D + off;
-            const f4 rq = a.rowq[at];
-            h8v q[NC];
+        const int rt0 = (a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0) + (by_rows ? w : 0), rt1 = (rows + 15) / 16;
+        const int stride = by_rows ? 4 : 1;
+        h8v q[NC];
+        f4 rq;
+        auto fetch = [&](int rt) {
+            const int64_t at = hd * a.rows16 + min(16 * min(rt, rt1 - 1) + i, rows - 1);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (qp + step * c);
-            const int lim = row < rows ? row_limit(a, len, n, rr / a.group) : 0;
+            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (a.qh + at * D + off + lo * (c & 1) + 64 * (c >> 1));
+            rq = a.rowq[at];
+        };
+        if (rt0 < rt1) fetch(rt0);
+        for (int rt = rt0; rt < rt1; rt += stride) {
+            const int row = 16 * rt + i;
             f4 sc[4];
 #pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) sc[b] = mfma32(kf[b][c], q[c], c ? sc[b] : (f4){0.f, 0.f, 0.f, 0.f});
+            const float factor = rq[0], top = rq[1], inv = row < rows ? rq[2] : 0.0f;
+            fetch(rt + stride);
+            // rows that see all of these slots: none is masked (a row past the last one has a finite row's scores)
+            const bool all = row_limit(a, len, n, 16 * rt / a.group) >= j0 + 64;
+            const int lim = row_limit(a, len, n, min(row, rows - 1) / a.group);
+#pragma unroll
             for (int b = 0; b < 4; ++b) {
-                sc[b] = (f4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < NC; ++c) sc[b] = mfma32(kf[b][c], q[c], sc[b]);
-            }
-#pragma unroll
-            for (int b = 0; b < 4; ++b)
+                const float f = ks[b] * factor;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(sc[b][e] * (ks[b] * rq[0]) - rq[1]);
-                    add[b][e] = fmaf(j0 + 16 * b + 4 * k + e < lim ? x : 0.0f, rq[2], add[b][e]);
+                    float x = __builtin_amdgcn_exp2f(sc[b][e] * f - top);
+                    if (!all) x = j0 + 16 * b + 4 * k + e < lim ? x : 0.0f;
+                    add[b][e] = fmaf(x, inv, add[b][e]);
                 }
+            }
         }
     }
 #pragma unroll
