@@ -193,8 +193,8 @@ def step_bench(args, cfg, w):
     head, batch 1) with the KV cache pre-filled at 512 positions with seeded
     N(0, 1) bfloat16-valued K/V rows, the new token at position 512.  Each
     call is one q3t_dev_talker_step (logits and hidden copied back to the
-    host): the persistent kernel's talker pass for an fp16 cache, the
-    multi-kernel step for a bfloat16 cache (--kv bf16).  Reports the mean wall
+    host): the persistent kernel's talker pass for a 16-bit cache, the
+    multi-kernel step for an 8-bit one (--kv i8).  Reports the mean wall
     time per step and the HIP event timings of the multi-kernel step's kernels
     for talker layer 0 at that context."""
     from qwen3_tts_amd.device import Device
@@ -202,8 +202,8 @@ def step_bench(args, cfg, w):
     n_kv = 512
     dev = Device(cfg, 0)
     dev.upload_weights(w)
-    if args.kv == "bf16":
-        dev.kv_set_type(30)
+    if args.kv != "f16":
+        dev.kv_set_type({"bf16": 30, "i8": 24}[args.kv])
     dev.kv_reserve(n_kv + 8)
 
     def bf16_bits(x):
@@ -212,7 +212,7 @@ def step_bench(args, cfg, w):
 
     for layer in range(cfg.n_layers):
         kv = [bf16_bits(rng.standard_normal((n_kv, cfg.n_kv_head, cfg.head_dim), dtype=np.float32)) for _ in range(2)]
-        if args.kv == "f16":    # the same bfloat16 values, held exactly in fp16
+        if args.kv != "bf16":   # the same bfloat16 values, held exactly in fp16 (quantised by an 8-bit cache)
             kv = [(b.astype(np.uint32) << np.uint32(16)).view(np.float32).astype(np.float16) for b in kv]
         dev.kv_write(layer, kv[0], kv[1])
     x = (rng.standard_normal(cfg.hidden_size) * 0.05).astype(np.float32)
@@ -228,13 +228,15 @@ def step_bench(args, cfg, w):
     kernels = {}
     names = {0: "gemv_gate_up_swiglu", 1: "gemv_qkv_rmsnorm", 2: "gemv_down_resid", 3: "gemv_wo_resid",
              4: "attention_decode"}
+    if args.kv == "i8":
+        del names[4]            # times the 16-bit caches' kernel
     for k_, nm in names.items():
         us, b = dev.time_kernel(k_, 100)
         kernels[nm] = {"avg_us": round(us, 3), "bytes": int(b), "gbs": round(b / us / 1e3, 1) if us > 0 else None}
     dev.close()
     wbytes = sum(a.nbytes for n_, (_, _, a) in w.tensors.items() if n_.startswith("talker.blk.")) + \
         w.tensors["talker.codec_head.weight"][2].nbytes
-    kvbytes = cfg.n_layers * cfg.n_kv_head * cfg.head_dim * 2 * 2 * (n_kv + 1)
+    kvbytes = cfg.n_layers * cfg.n_kv_head * cfg.head_dim * 2 * (1 if args.kv == "i8" else 2) * (n_kv + 1)
     print(json.dumps({
         "metric": "talker decode step latency (KV 512)", "value": round(dt * 1e3, 4), "unit": "ms",
         "n_gpus": 1, "steps": steps, "warmup": max(args.warmup, 1), "ms_per_step": round(dt * 1e3, 4),
@@ -496,7 +498,7 @@ def main():
                     help="instead of the frame loop, time one talker prefill of this many rows (Q8_0: int8 MFMA path)")
     ap.add_argument("--talker-step", action="store_true",
                     help="instead of the frame loop, time one talker decode step at a 512-position KV cache")
-    ap.add_argument("--kv", default="f16", choices=["f16", "bf16"], help="--talker-step: talker KV cache type")
+    ap.add_argument("--kv", default="f16", choices=["f16", "bf16", "i8"], help="--talker-step: talker KV cache type")
     ap.add_argument("--long", action="store_true",
                     help="instead of the short-prompt greedy loop, time long-context sampled decode after a long prefill")
     ap.add_argument("--long-prompt", type=int, default=2048, help="text ids of the --long prefill")

@@ -5,6 +5,7 @@
 // every entry point fails with an error.
 
 #include "../../include/q3t_dev.h"
+#include "../../include/q3t_kv8.h"
 #include "q3t_kernels.h"
 #include "q3t_frame_kernel.h"
 #include "q3t_prefill.h"
@@ -152,6 +153,17 @@ struct q3t_dev {
     // caches
     uint16_t * kc = nullptr, * vc = nullptr; int32_t n_ctx = 0;
     bool kv_bf16 = false;          // talker cache elements are bfloat16 (q3t_dev_kv_set_type), else fp16
+    // 8-bit talker cache (q3t_dev_kv_set_type I8; kc and vc are null then): a layer is kv8_layer bytes of codes, scales
+    // and drawn weights; positions and slots part once slots have been evicted
+    bool kv_i8 = false;
+    unsigned char * kv8 = nullptr, * kv8_spare = nullptr; size_t kv8_layer = 0;
+    int32_t kv8_evicted = 0, kv8_floor = 0;   // position p is slot p - evicted, from position `floor` on
+    int32_t * kv8_at = nullptr;               // device: evicted; slot and length of the step's row
+    double * kv8_freq = nullptr; float kv8_mscale = 1.0f;
+    int32_t kv8_scaling = 0, kv8_trained = 0; double kv8_factor = 1.0;
+    uint16_t * kv8_q = nullptr; size_t kv8_q_cap = 0;       // rotated q rows in fp16
+    unsigned char * kv8_ws = nullptr; size_t kv8_ws_cap = 0;
+    int32_t * kv8_kept = nullptr; size_t kv8_kept_cap = 0;
     uint16_t * cpk = nullptr, * cpv = nullptr;
     float * rope_cos = nullptr, * rope_sin = nullptr, * cp_rope_cos = nullptr, * cp_rope_sin = nullptr;
     int32_t rope_rows = 0;
@@ -197,6 +209,7 @@ struct q3t_dev {
     double run_us = 0.0;
     int64_t run_frames = 0;
     int32_t host_emitted = 0;
+    int32_t frames_base = 0;           // talker position of the loop's first frame
     int32_t frames_launched = 0;
     int32_t frames_max = 0;
     bool frames_ready = false;
@@ -621,16 +634,147 @@ void layer_single(q3t_dev * c, const LayerDev & L, const float * xin, int d, int
     layer_tail(c, L, xin, 1, d, ffn, true);
 }
 
+// ------------------------------------------------------ 8-bit talker cache
+int kv8_slots(const q3t_dev * c) { return (c->n_ctx + Q3T_KV8_BLOCK - 1) / Q3T_KV8_BLOCK * Q3T_KV8_BLOCK; }
+
+// One layer's cache at `base`: codes of K and V, their scales, drawn weights.
+q3t_kv8 kv8_cache(const q3t_dev * c, unsigned char * base) {
+    const q3t_config & g = c->cfg;
+    const int64_t slots = kv8_slots(c), H = g.n_kv_head, blocks = slots / Q3T_KV8_BLOCK;
+    q3t_kv8 k{};
+    k.k = (int8_t *) base;
+    k.v = k.k + H * slots * g.head_dim;
+    k.ks = (float *) (k.v + H * slots * g.head_dim);
+    k.vs = k.ks + H * blocks;
+    k.acc = k.vs + H * blocks;
+    k.head = slots * g.head_dim; k.seq = H * k.head;
+    k.scale_head = blocks; k.scale_seq = H * blocks;
+    k.acc_head = slots; k.acc_seq = H * slots;
+    k.n_seq = 1; k.n_kv_head = (int32_t) H; k.n_slots = (int32_t) slots; k.head_dim = g.head_dim;
+    return k;
+}
+
+q3t_kv8_attend_args kv8_attend_args(const q3t_dev * c, int n) {
+    const q3t_config & g = c->cfg;
+    q3t_kv8_attend_args a{};
+    a.q = c->kv8_q; a.q_row = (int64_t) g.n_head * g.head_dim; a.q_head = g.head_dim; a.q_type = Q3T_TYPE_F16;
+    a.o_row = a.q_row; a.o_head = g.head_dim;
+    a.n_rows = n; a.n_head = g.n_head; a.causal = 1; a.weights = 1;
+    a.scale = 1.0f / std::sqrt((float) g.head_dim);
+    return a;
+}
+
+int kv8_fail(q3t_dev * c) { return fail(c, std::string("8-bit cache: ") + q3t_kv8_last_error()); }
+
+// Work buffers of calls of up to n rows.
+int ensure_kv8(q3t_dev * c, int n) {
+    const q3t_config & g = c->cfg;
+    const size_t q = (size_t) n * g.n_head * g.head_dim;
+    if (q > c->kv8_q_cap) {
+        dev_free(c, c->kv8_q);
+        c->kv8_q = nullptr; c->kv8_q_cap = 0;
+        if (dev_alloc_t(c, &c->kv8_q, q)) return -1;
+        c->kv8_q_cap = q;
+        drop_graph(c);
+    }
+    const q3t_kv8 k = kv8_cache(c, c->kv8);
+    // a short call may be split over more of the cache than a long one
+    size_t ws = 0;
+    for (int r : {1, 2, 4, n}) {
+        if (r > n) continue;
+        const q3t_kv8_attend_args a = kv8_attend_args(c, r);
+        const int64_t need = q3t_kv8_attend_ws(&k, &a);
+        if (need < 0) return kv8_fail(c);
+        ws = std::max(ws, (size_t) need);
+    }
+    if (ws > c->kv8_ws_cap) {
+        dev_free(c, c->kv8_ws);
+        c->kv8_ws = nullptr; c->kv8_ws_cap = 0;
+        if (dev_alloc_t(c, &c->kv8_ws, ws)) return -1;
+        c->kv8_ws_cap = ws;
+        drop_graph(c);
+    }
+    return 0;
+}
+
+// The slot of the step at st->talker_pos and the cache's length with it; none
+// once the frame loop is done.
+__global__ void k_kv8_place(const FrameState * st, int32_t * at) {
+    const int slot = st->talker_pos - at[0];
+    at[1] = st->done ? -1 : slot;
+    at[2] = st->done ? 0 : slot + 1;
+}
+
+// Attention of n rows of layer il over the 8-bit cache: q and k normed and
+// rotated, K and V stored, attention with the weights drawn.  qkv: rows of q |
+// k | v (k is rotated in place); out: [n][n_head * head_dim] of o_type.  step:
+// one row at the slot that k_kv8_place left (position st->talker_pos), else
+// positions n_past ...
+int kv8_attention(q3t_dev * c, const LayerDev & L, int il, float * qkv, int n, bool step, int n_past, void * out,
+                  int o_type) {
+    const q3t_config & g = c->cfg;
+    const int64_t qd = (int64_t) g.n_head * g.head_dim, kd = (int64_t) g.n_kv_head * g.head_dim, w = qd + 2 * kd;
+    const q3t_kv8 cache = kv8_cache(c, c->kv8 + (size_t) il * c->kv8_layer);
+    const q3t_kv8_rope_rows rows[2] = {
+        {qkv, c->kv8_q, w, g.head_dim, qd, g.head_dim, L.q_norm, g.n_head, Q3T_TYPE_F32, Q3T_TYPE_F16},
+        {qkv + qd, qkv + qd, w, g.head_dim, w, g.head_dim, L.k_norm, g.n_kv_head, Q3T_TYPE_F32, Q3T_TYPE_F32}};
+    const int slot = n_past - c->kv8_evicted;
+    q3t_kv8_attend_args a = kv8_attend_args(c, n);
+    a.out = out; a.o_type = o_type;
+    a.lens = step ? c->kv8_at + 2 : nullptr; a.len0 = step ? 0 : slot + n;
+    if (q3t_kv8_rope(c->device, rows, 2, n, g.head_dim, g.head_dim, 0, step ? &c->st->talker_pos : nullptr,
+                     step ? 0 : n_past, c->kv8_freq, c->kv8_mscale, g.rms_eps, c->stream) ||
+        q3t_kv8_append(c->device, &cache, qkv + qd, qkv + qd + kd, Q3T_TYPE_F32, 0, w, g.head_dim, n,
+                       step ? c->kv8_at + 1 : nullptr, step ? 0 : slot, nullptr, c->stream) ||
+        q3t_kv8_attend(c->device, &cache, &a, c->kv8_ws, (int64_t) c->kv8_ws_cap, c->stream))
+        return kv8_fail(c);
+    return 0;
+}
+
+// Whether positions n_past .. n_past + n - 1 can be written: an 8-bit cache
+// has slots for them behind what an eviction kept (position 0 starts the cache
+// anew), any other one holds them all.
+int check_room(q3t_dev * c, int32_t n_past, int32_t n) {
+    if (c->kv_i8 && n_past == 0 && (c->kv8_evicted || c->kv8_floor)) {
+        c->kv8_evicted = c->kv8_floor = 0;
+        HIP_OK(hipMemsetAsync(c->kv8_at, 0, 4 * sizeof(int32_t), c->stream));
+    }
+    if (c->kv_i8 && n_past >= 0 && n_past < c->kv8_floor) return fail(c, "position precedes the cache's last eviction");
+    if (n_past < 0 || (int64_t) n_past - c->kv8_evicted + n > c->n_ctx) return fail(c, "Context length exceeded");
+    return 0;
+}
+
+// The talker's rotary frequencies (q3t_dev_set_rope_scaling).
+int kv8_freqs(q3t_dev * c) {
+    const q3t_config & g = c->cfg;
+    std::vector<double> f(g.head_dim / 2);
+    if (q3t_kv8_rope_freqs(g.head_dim, g.rope_theta, c->kv8_scaling, c->kv8_factor, c->kv8_trained, f.data())) return kv8_fail(c);
+    HIP_OK(hipMemcpy(c->kv8_freq, f.data(), f.size() * sizeof(double), hipMemcpyHostToDevice));
+    return 0;
+}
+
 // Talker forward of nt (<= 4) tokens whose input rows are `xin`.  The codec
 // head runs on the last row when `head` is set (normed hidden of that row ->
 // c->hidden, logits -> c->logits).  A single-token step (`step`) writes the
 // post-softmax rows of layer c->attn_layer to c->probs when capture is on.
-void talker_chunk(q3t_dev * c, const float * xin, int nt, const int32_t * pos_ptr, int pos_const, bool head,
-                  bool step = false) {
+int talker_chunk(q3t_dev * c, const float * xin, int nt, const int32_t * pos_ptr, int pos_const, bool head,
+                 bool step = false) {
     const q3t_config & g = c->cfg;
     const int d = g.hidden_size;
     const size_t lstride = (size_t) g.n_kv_head * c->n_ctx * g.head_dim;
-    for (int il = 0; il < g.n_layers; ++il)
+    if (c->kv_i8 && step) hipLaunchKernelGGL(k_kv8_place, dim3(1), dim3(1), 0, c->stream, (const FrameState *) c->st, c->kv8_at);
+    for (int il = 0; il < g.n_layers && c->kv_i8; ++il) {
+        const LayerDev & L = c->talker[il];
+        const float * x = il == 0 ? xin : c->xa;
+        const int qkvd = (g.n_head + 2 * g.n_kv_head) * g.head_dim;
+        GemvSpec s{};
+        s.w = weight_of(L.qkv); s.rows = qkvd; s.K = d; s.x = x; s.x_stride = d; s.norm_w = L.attn_norm;
+        s.y = c->qkv; s.y_stride = qkvd;
+        gemv(c, s, nt);
+        if (kv8_attention(c, L, il, c->qkv, nt, step, pos_const, c->attn, Q3T_TYPE_F32)) return -1;
+        layer_tail(c, L, x, nt, d, g.ffn_size, false);
+    }
+    for (int il = 0; il < g.n_layers && !c->kv_i8; ++il)
         layer(c, c->talker[il], il == 0 ? xin : c->xa, nt, d, g.ffn_size, c->kc + il * lstride, c->vc + il * lstride,
               c->n_ctx, c->rope_cos, c->rope_sin, pos_ptr, pos_const, false,
               step && nt == 1 && il == c->attn_layer ? c->probs : nullptr);
@@ -641,6 +785,7 @@ void talker_chunk(q3t_dev * c, const float * xin, int nt, const int32_t * pos_pt
         h.hidden_out = c->hidden; h.hidden_stride = d; h.y = c->logits; h.y_stride = g.codec_vocab;
         gemv(c, h, 1);
     }
+    return 0;
 }
 
 SampleArgs sample_args(q3t_dev * c, int mode, int group) {
@@ -723,12 +868,12 @@ void code_pred_single(q3t_dev * c, SingleInArgs in) {
 // code-predictor prefill rows), the code predictor (emits the frame and
 // gathers the step embedding), the talker step.  Every kernel reads its
 // dynamic inputs from c->st.
-void frame_seq(q3t_dev * c) {
+int frame_seq(q3t_dev * c) {
     SampleArgs sa = sample_args(c, 0, 0);
     sa.open_frame = 1;
     hipLaunchKernelGGL(k_sample, dim3(1), dim3(kSampleThreads), 0, c->stream, sa);
     code_pred_seq(c, true);
-    talker_chunk(c, c->stage, 1, &c->st->talker_pos, 0, true, true);
+    return talker_chunk(c, c->stage, 1, &c->st->talker_pos, 0, true, true);
 }
 
 int set_state(q3t_dev * c, const FrameState & s) {
@@ -749,7 +894,7 @@ int ensure_stage(q3t_dev * c, int rows) {
 
 int check_ready(q3t_dev * c) {
     if (resolve(c)) return -1;
-    if (!c->kc) return fail(c, "KV cache not reserved");
+    if (!c->kc && !c->kv8) return fail(c, "KV cache not reserved");
     return 0;
 }
 
@@ -865,8 +1010,8 @@ int build_cp_tab(q3t_dev * c);   // below, with the prefill helpers it uses
 
 int fk_prepare(q3t_dev * c) {
     c->fk_ok = false;
-    // attention capture runs the multi-kernel step
-    if (c->fk_refused || c->attn_layer >= 0) return 0;
+    // attention capture and the 8-bit cache run the multi-kernel step
+    if (c->fk_refused || c->attn_layer >= 0 || c->kv_i8) return 0;
     if (const char * e = std::getenv("Q3T_FRAME_KERNEL")) if (e[0] == '0') return 0;
     const q3t_config & g = c->cfg;
     const int qd = g.n_head * g.head_dim, kd = g.n_kv_head * g.head_dim, qkvd = qd + 2 * kd;
@@ -1134,9 +1279,13 @@ int ensure_frame_graph(q3t_dev * c) {
     if (c->frame_exec) return 0;
     HIP_OK(hipStreamSynchronize(c->stream));
     HIP_OK(hipStreamBeginCapture(c->stream, hipStreamCaptureModeThreadLocal));
-    frame_seq(c);
+    const int rc = frame_seq(c);
     hipGraph_t graph = nullptr;
     HIP_OK(hipStreamEndCapture(c->stream, &graph));
+    if (rc) {
+        (void) hipGraphDestroy(graph);
+        return -1;
+    }
     c->frame_graph = graph;
     HIP_OK(hipGraphInstantiate(&c->frame_exec, graph, nullptr, nullptr, 0));
     return 0;
@@ -1411,15 +1560,17 @@ int q3t_dev_kv_reserve(q3t_dev * c, int32_t n_ctx) {
     int max_lds = 0;
     HIP_OK(hipDeviceGetAttribute(&max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock, c->device));
     const size_t need_att = attn_lds_bytes(n_ctx), need_pf = pf::attn_rows_lds_bytes(n_ctx);
-    if (std::max(need_att, need_pf) > (size_t) max_lds) {
+    if (!c->kv_i8 && std::max(need_att, need_pf) > (size_t) max_lds) {
         char msg[160];
         snprintf(msg, sizeof msg, "n_ctx %d needs %zu bytes of LDS for the decode attention; the device has %d",
                  (int) n_ctx, std::max(need_att, need_pf), max_lds);
         return fail(c, msg);
     }
-    HIP_OK(hipFuncSetAttribute((const void *) k_attention, hipFuncAttributeMaxDynamicSharedMemorySize, (int) need_att));
-    HIP_OK(hipFuncSetAttribute((const void *) pf::k_attn_rows, hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int) need_pf));
+    if (!c->kv_i8) {
+        HIP_OK(hipFuncSetAttribute((const void *) k_attention, hipFuncAttributeMaxDynamicSharedMemorySize, (int) need_att));
+        HIP_OK(hipFuncSetAttribute((const void *) pf::k_attn_rows, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                   (int) need_pf));
+    }
     HIP_OK(hipStreamSynchronize(c->stream));
     drop_graph(c);
     drop_stream_graph(c);
@@ -1429,19 +1580,39 @@ int q3t_dev_kv_reserve(q3t_dev * c, int32_t n_ctx) {
     c->kc = c->vc = c->cpk = c->cpv = nullptr;
     c->probs = nullptr;
     c->probs_cap = 0;
+    for (void * p : {(void *) c->kv8, (void *) c->kv8_spare, (void *) c->kv8_q, (void *) c->kv8_ws, (void *) c->kv8_kept})
+        dev_free(c, p);
+    c->kv8 = c->kv8_spare = c->kv8_ws = nullptr;
+    c->kv8_q = nullptr; c->kv8_kept = nullptr;
+    c->kv8_q_cap = c->kv8_ws_cap = c->kv8_kept_cap = 0;
+    c->kv8_evicted = c->kv8_floor = 0;
+    c->n_ctx = 0;
     const size_t kv = (size_t) g.n_layers * g.n_kv_head * n_ctx * g.head_dim;
     const size_t ckv = (size_t) g.cp_layers * g.n_kv_head * 16 * g.head_dim;
-    if (dev_alloc_t(c, &c->kc, kv) || dev_alloc_t(c, &c->vc, kv) || dev_alloc_t(c, &c->cpk, ckv) ||
-        dev_alloc_t(c, &c->cpv, ckv) || dev_alloc_t(c, &c->probs, (size_t) g.n_head * n_ctx))
-        return -1;
-    c->probs_cap = n_ctx;
-    HIP_OK(hipMemsetAsync(c->kc, 0, kv * 2, c->stream));
-    HIP_OK(hipMemsetAsync(c->vc, 0, kv * 2, c->stream));
+    if (dev_alloc_t(c, &c->cpk, ckv) || dev_alloc_t(c, &c->cpv, ckv)) return -1;
+    if (c->kv_i8) {
+        c->n_ctx = n_ctx;
+        const size_t slots = kv8_slots(c), H = g.n_kv_head;
+        c->kv8_layer = (H * slots * (2 * g.head_dim + 4) + 2 * H * (slots / Q3T_KV8_BLOCK) * 4 + 255) / 256 * 256;
+        if (dev_alloc_t(c, &c->kv8, g.n_layers * c->kv8_layer) ||
+            (!c->kv8_at && dev_alloc_t(c, &c->kv8_at, 4)) || (!c->kv8_freq && dev_alloc_t(c, &c->kv8_freq, g.head_dim / 2)))
+            return -1;
+        HIP_OK(hipMemsetAsync(c->kv8, 0, g.n_layers * c->kv8_layer, c->stream));
+        HIP_OK(hipMemsetAsync(c->kv8_at, 0, 4 * sizeof(int32_t), c->stream));
+        if (kv8_freqs(c) || ensure_kv8(c, 4)) return -1;
+    } else {
+        if (dev_alloc_t(c, &c->kc, kv) || dev_alloc_t(c, &c->vc, kv) || dev_alloc_t(c, &c->probs, (size_t) g.n_head * n_ctx))
+            return -1;
+        c->probs_cap = n_ctx;
+        HIP_OK(hipMemsetAsync(c->kc, 0, kv * 2, c->stream));
+        HIP_OK(hipMemsetAsync(c->vc, 0, kv * 2, c->stream));
+    }
     HIP_OK(hipMemsetAsync(c->cpk, 0, ckv * 2, c->stream));
     HIP_OK(hipMemsetAsync(c->cpv, 0, ckv * 2, c->stream));
     // RoPE tables: theta_i = pos * base^(-2i/hd) by cumulative fp32 product
     // (ggml_rope_cache_init), cos/sin from the C library, once per context.
-    const int rows = std::max(n_ctx, 16), half = g.head_dim / 2;
+    // (an 8-bit cache's talker rotates by any position: its table holds the code predictor's positions alone)
+    const int rows = c->kv_i8 ? 16 : std::max(n_ctx, 16), half = g.head_dim / 2;
     std::vector<float> tc((size_t) rows * half), ts((size_t) rows * half), cc((size_t) rows * half), cs((size_t) rows * half);
     auto fill = [&](float base, std::vector<float> & co, std::vector<float> & si) {
         const float theta_scale = std::pow(base, -2.0f / (float) g.head_dim);
@@ -1471,7 +1642,7 @@ int q3t_dev_kv_reserve(q3t_dev * c, int32_t n_ctx) {
         HIP_OK(hipDeviceGetAttribute(&max_lds, hipDeviceAttributeMaxSharedMemoryPerBlock, c->device));
         const int G = g.n_kv_head > 0 ? g.n_head / g.n_kv_head : 0;
         c->gqa_lds_ok = false;
-        if (G == 1 || G == 2 || G == 4) {
+        if (!c->kv_i8 && (G == 1 || G == 2 || G == 4)) {
             const size_t al = ms::attn_gqa_lds_bytes(1, n_ctx);
             if (al <= (size_t) max_lds) {
                 HIP_OK(hipFuncSetAttribute((const void *) ms::k_attn_gqa<1>, hipFuncAttributeMaxDynamicSharedMemorySize,
@@ -1491,10 +1662,13 @@ int32_t q3t_dev_kv_capacity(const q3t_dev * c) { return c ? c->n_ctx : 0; }
 
 int q3t_dev_kv_set_type(q3t_dev * c, int32_t type) {
     if (!c) return -1;
-    if (type != Q3T_TYPE_F16 && type != Q3T_TYPE_BF16) return fail(c, "talker KV type must be F16 or BF16");
-    const bool bf = type == Q3T_TYPE_BF16;
-    if (bf == c->kv_bf16) return 0;
+    if (type != Q3T_TYPE_F16 && type != Q3T_TYPE_BF16 && type != Q3T_TYPE_I8)
+        return fail(c, "talker KV type must be F16, BF16 or I8");
+    const bool bf = type == Q3T_TYPE_BF16, i8 = type == Q3T_TYPE_I8;
+    if (bf == c->kv_bf16 && i8 == c->kv_i8) return 0;
+    if (i8 && c->attn_layer >= 0) return fail(c, "attention capture needs an F16 or BF16 talker cache");
     c->kv_bf16 = bf;
+    c->kv_i8 = i8;
     c->fk_ok = false;
     c->fk_args_ok = false;
     c->frames_ready = false;
@@ -1505,6 +1679,7 @@ int q3t_dev_kv_set_type(q3t_dev * c, int32_t type) {
 int q3t_dev_set_attn_capture(q3t_dev * c, int32_t layer) {
     if (!c) return -1;
     if (layer < -1 || layer >= c->cfg.n_layers) return fail(c, "attention capture layer out of range");
+    if (layer >= 0 && c->kv_i8) return fail(c, "attention capture needs an F16 or BF16 talker cache");
     HIP_OK(hipSetDevice(c->device));
     HIP_OK(hipStreamSynchronize(c->stream));
     if (layer != c->attn_layer) {
@@ -1536,9 +1711,25 @@ int q3t_dev_attn_row(q3t_dev * c, int32_t index, float * out, int64_t cap, int32
 int q3t_dev_kv_write(q3t_dev * c, int32_t layer, int32_t n_pos, const uint16_t * k, const uint16_t * v) {
     if (!c || !k || !v) return -1;
     const q3t_config & g = c->cfg;
-    if (!c->kc) return fail(c, "KV cache not reserved");
+    if (!c->kc && !c->kv8) return fail(c, "KV cache not reserved");
     if (layer < 0 || layer >= g.n_layers || n_pos < 0 || n_pos > c->n_ctx) return fail(c, "kv_write out of range");
     HIP_OK(hipSetDevice(c->device));
+    if (c->kv_i8) {
+        if (check_room(c, 0, n_pos)) return -1;
+        const size_t row = (size_t) g.n_kv_head * g.head_dim, bytes = n_pos * row * 2;
+        uint16_t * d = nullptr;
+        if (dev_alloc_t(c, &d, 2 * n_pos * row)) return -1;
+        const q3t_kv8 cache = kv8_cache(c, c->kv8 + (size_t) layer * c->kv8_layer);
+        int rc = hipMemcpyAsync(d, k, bytes, hipMemcpyHostToDevice, c->stream) == hipSuccess &&
+                         hipMemcpyAsync(d + n_pos * row, v, bytes, hipMemcpyHostToDevice, c->stream) == hipSuccess
+                     ? 0 : fail(c, "kv_write: copy failed");
+        if (!rc && q3t_kv8_append(c->device, &cache, d, d + n_pos * row, Q3T_TYPE_F16, 0, (int64_t) row, g.head_dim, n_pos,
+                                  nullptr, 0, nullptr, c->stream))
+            rc = kv8_fail(c);
+        if (hipStreamSynchronize(c->stream) != hipSuccess && !rc) rc = fail(c, "kv_write failed");
+        dev_free(c, d);
+        return rc;
+    }
     const size_t lstride = (size_t) g.n_kv_head * c->n_ctx * g.head_dim;
     std::vector<uint16_t> tk((size_t) n_pos * g.head_dim);
     for (int h = 0; h < g.n_kv_head; ++h) {
@@ -1552,6 +1743,85 @@ int q3t_dev_kv_write(q3t_dev * c, int32_t layer, int32_t n_pos, const uint16_t *
         }
     }
     return 0;
+}
+
+int q3t_dev_kv_read(q3t_dev * c, int32_t layer, int32_t slot0, int32_t n, float * k, float * v, float * weight) {
+    if (!c) return -1;
+    const q3t_config & g = c->cfg;
+    if (!c->kv_i8 || !c->kv8) return fail(c, "kv_read needs a reserved I8 cache");
+    if (layer < 0 || layer >= g.n_layers || slot0 < 0 || n < 0 || (int64_t) slot0 + n > c->n_ctx) return fail(c, "kv_read out of range");
+    if (!n) return 0;
+    HIP_OK(hipSetDevice(c->device));
+    const q3t_kv8 cache = kv8_cache(c, c->kv8 + (size_t) layer * c->kv8_layer);
+    const size_t cells = (size_t) n * g.n_kv_head * g.head_dim;
+    float * d = nullptr;
+    if (dev_alloc_t(c, &d, 2 * cells)) return -1;
+    int rc = q3t_kv8_read(c->device, &cache, nullptr, slot0, n, Q3T_TYPE_F32, d, d + cells, c->stream) ? kv8_fail(c) : 0;
+    auto copy = [&](void * to, const void * from, size_t bytes) {
+        if (!rc && to && hipMemcpyAsync(to, from, bytes, hipMemcpyDeviceToHost, c->stream) != hipSuccess)
+            rc = fail(c, "kv_read: copy failed");
+    };
+    copy(k, d, cells * 4);
+    copy(v, d + cells, cells * 4);
+    for (int h = 0; h < g.n_kv_head && weight; ++h) copy(weight + (size_t) h * n, cache.acc + h * cache.acc_head + slot0, (size_t) n * 4);
+    if (hipStreamSynchronize(c->stream) != hipSuccess && !rc) rc = fail(c, "kv_read failed");
+    dev_free(c, d);
+    return rc;
+}
+
+int q3t_dev_kv_evict(q3t_dev * c, int32_t n_past, int32_t n_keep, int32_t n_sink, int32_t n_recent, int32_t * kept_out) {
+    if (!c) return -1;
+    const q3t_config & g = c->cfg;
+    if (!c->kv_i8 || !c->kv8) return fail(c, "kv_evict needs a reserved I8 cache");
+    if (n_past < c->kv8_floor || n_past - c->kv8_evicted > c->n_ctx) return fail(c, "kv_evict: n_past is not this cache's");
+    if (n_keep < 1 || n_keep > c->n_ctx || n_sink < 0 || n_recent < 0 || (int64_t) n_sink + n_recent > n_keep)
+        return fail(c, "kv_evict: n_keep must be 1 to n_ctx and at least n_sink + n_recent");
+    HIP_OK(hipSetDevice(c->device));
+    const int len = n_past - c->kv8_evicted;
+    const size_t rows = (size_t) g.n_kv_head * n_keep;
+    if (len <= n_keep) {
+        for (size_t i = 0; kept_out && i < rows * g.n_layers; ++i) kept_out[i] = (int32_t) (i % n_keep) < len ? (int32_t) (i % n_keep) : -1;
+        return 0;
+    }
+    if (!c->kv8_spare) {
+        if (dev_alloc_t(c, &c->kv8_spare, c->kv8_layer)) return -1;
+        HIP_OK(hipMemsetAsync(c->kv8_spare, 0, c->kv8_layer, c->stream));
+    }
+    if (rows > c->kv8_kept_cap) {
+        dev_free(c, c->kv8_kept);
+        c->kv8_kept = nullptr; c->kv8_kept_cap = 0;
+        if (dev_alloc_t(c, &c->kv8_kept, rows)) return -1;
+        c->kv8_kept_cap = rows;
+    }
+    const q3t_kv8 to = kv8_cache(c, c->kv8_spare);
+    for (int il = 0; il < g.n_layers; ++il) {
+        unsigned char * base = c->kv8 + (size_t) il * c->kv8_layer;
+        const q3t_kv8 from = kv8_cache(c, base);
+        if (q3t_kv8_evict(c->device, &from, &to, nullptr, len, n_keep, n_sink, n_recent, c->kv8_kept, nullptr, c->stream))
+            return kv8_fail(c);
+        // back to the layer's own place, which captured frames address
+        HIP_OK(hipMemcpyAsync(base, c->kv8_spare, c->kv8_layer, hipMemcpyDeviceToDevice, c->stream));
+        if (kept_out)
+            HIP_OK(hipMemcpyAsync(kept_out + il * rows, c->kv8_kept, rows * sizeof(int32_t), hipMemcpyDeviceToHost, c->stream));
+    }
+    c->kv8_evicted = n_past - n_keep;
+    c->kv8_floor = n_past;
+    HIP_OK(hipMemcpyAsync(c->kv8_at, &c->kv8_evicted, sizeof(int32_t), hipMemcpyHostToDevice, c->stream));
+    return sync(c);
+}
+
+int q3t_dev_set_rope_scaling(q3t_dev * c, int32_t scaling, double factor, int32_t n_trained, float mscale) {
+    if (!c) return -1;
+    if (!c->kv_i8) return fail(c, "rotary scaling needs an I8 talker cache");
+    if (!(mscale > 0.0f) || !std::isfinite(mscale)) return fail(c, "mscale must be positive");
+    std::vector<double> f(c->cfg.head_dim / 2);
+    if (q3t_kv8_rope_freqs(c->cfg.head_dim, c->cfg.rope_theta, scaling, factor, n_trained, f.data())) return kv8_fail(c);
+    c->kv8_scaling = scaling; c->kv8_factor = factor; c->kv8_trained = n_trained;
+    HIP_OK(hipSetDevice(c->device));
+    HIP_OK(hipStreamSynchronize(c->stream));
+    if (mscale != c->kv8_mscale) drop_graph(c);     // captured frames hold it
+    c->kv8_mscale = mscale;
+    return c->kv8_freq ? kv8_freqs(c) : 0;
 }
 
 }  // extern "C"
@@ -1747,7 +2017,7 @@ int rows_check(q3t_dev * c) {
 // history, and an attention launch whose LDS holds a row's scores.
 // Q3T_PREFILL_MFMA (either value) keeps the other paths.
 bool rows_prefill(q3t_dev * c, int n, int n_past) {
-    if (n < (n_past < kRowsTwo ? 3 : 2) || n >= pf::kAT || std::getenv("Q3T_PREFILL_MFMA") || !c->gqa_lds_ok)
+    if (n < (n_past < kRowsTwo ? 3 : 2) || n >= pf::kAT || std::getenv("Q3T_PREFILL_MFMA") || !c->gqa_lds_ok || c->kv_i8)
         return false;
     const q3t_config & g = c->cfg;
     const int64_t weights = (int64_t) g.hidden_size * ((2 * g.n_head + 2 * g.n_kv_head) * g.head_dim + 3 * g.ffn_size);
@@ -2119,10 +2389,14 @@ int prefill_f16(q3t_dev * c, int n, int n_past) {
         hipLaunchKernelGGL(pf::k_rmsnorm_rows_h16, dim3(n), dim3(kBlock), 0, c->stream, x, L.attn_norm, g.rms_eps, d,
                            c->pf_h);
         pf_gemm_h16(c, L.qkv, qkvd, d, n, c->pf_h, nullptr, d, nullptr, c->pf_qkv, nullptr, 0);
-        hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
-                           qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
-                           kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
-        if (pf_attention(c, L, kc, vc, n, n_past, true)) return -1;
+        if (c->kv_i8) {
+            if (kv8_attention(c, L, il, c->pf_qkv, n, false, n_past, c->pf_h, Q3T_TYPE_F16)) return -1;
+        } else {
+            hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
+                               qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
+                               kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
+            if (pf_attention(c, L, kc, vc, n, n_past, true)) return -1;
+        }
         pf_gemm_h16(c, L.wo, d, qd, n, c->pf_h, nullptr, qd, nullptr, c->pf_xb, x, d);
         hipLaunchKernelGGL(pf::k_rmsnorm_rows_h16, dim3(n), dim3(kBlock), 0, c->stream, (const float *) c->pf_xb,
                            L.ffn_norm, g.rms_eps, d, c->pf_h);
@@ -2139,10 +2413,14 @@ int prefill_f16(q3t_dev * c, int n, int n_past) {
         uint16_t * vc = c->vc + il * lstride;
         hipLaunchKernelGGL(k_rmsnorm_rows, dim3(n), dim3(kBlock), 0, c->stream, x, L.attn_norm, g.rms_eps, d, c->pf_f);
         pf_gemm_f16(c, L.qkv, qkvd, d, n, c->pf_f, d, false, c->pf_qkv, nullptr, 0);
-        hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
-                           qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
-                           kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
-        if (pf_attention(c, L, kc, vc, n, n_past, false)) return -1;
+        if (c->kv_i8) {
+            if (kv8_attention(c, L, il, c->pf_qkv, n, false, n_past, c->pf_att, Q3T_TYPE_F32)) return -1;
+        } else {
+            hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
+                               qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
+                               kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
+            if (pf_attention(c, L, kc, vc, n, n_past, false)) return -1;
+        }
         pf_gemm_f16(c, L.wo, d, qd, n, c->pf_att, qd, false, c->pf_xb, x, d);
         hipLaunchKernelGGL(k_rmsnorm_rows, dim3(n), dim3(kBlock), 0, c->stream, (const float *) c->pf_xb, L.ffn_norm,
                            g.rms_eps, d, c->pf_f);
@@ -2177,10 +2455,14 @@ int prefill_mfma(q3t_dev * c, int n, int n_past) {
         uint16_t * vc = c->vc + il * lstride;
         pf_quant(c, x, n, d, L.attn_norm);
         pf_gemm(c, L.qkv, qkvd, d, n, c->pf_qkv, nullptr);
-        hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
-                           qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
-                           kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
-        if (pf_attention(c, L, kc, vc, n, n_past, false)) return -1;
+        if (c->kv_i8) {
+            if (kv8_attention(c, L, il, c->pf_qkv, n, false, n_past, c->pf_att, Q3T_TYPE_F32)) return -1;
+        } else {
+            hipLaunchKernelGGL(pf::k_kv_rows, dim3(n, (g.n_kv_head + 3) / 4), dim3(kBlock), 0, c->stream, (const float *) c->pf_qkv,
+                               qkvd, qd, kd, L.k_norm, g.rms_eps, (const float *) c->rope_cos, (const float *) c->rope_sin,
+                               kc, vc, c->n_ctx, n_past, c->kv_bf16 ? 1 : 0);
+            if (pf_attention(c, L, kc, vc, n, n_past, false)) return -1;
+        }
         pf_quant(c, c->pf_att, n, qd, nullptr);
         pf_gemm(c, L.wo, d, qd, n, c->pf_xb, x);
         pf_quant(c, c->pf_xb, n, d, L.ffn_norm);
@@ -2448,7 +2730,8 @@ int q3t_dev_prefill(q3t_dev * c, const float * embd, int32_t n, int32_t n_past, 
     if (n <= 0) return fail(c, "n_tokens must be > 0");
     HIP_OK(hipSetDevice(c->device));
     if (check_ready(c)) return -1;
-    if (n_past < 0 || n_past + n > c->n_ctx) return fail(c, "Context length exceeded");
+    if (check_room(c, n_past, n)) return -1;
+    if (c->kv_i8 && ensure_kv8(c, n)) return -1;
     const q3t_config & g = c->cfg;
     const int d = g.hidden_size;
     if (ensure_stage(c, n)) return -1;
@@ -2478,7 +2761,7 @@ int q3t_dev_prefill(q3t_dev * c, const float * embd, int32_t n, int32_t n_past, 
         const int left = n - t0;
         const int nt = left >= 4 ? 4 : left >= 2 ? 2 : 1;
         const bool last = t0 + nt == n;
-        talker_chunk(c, c->stage + (size_t) t0 * d, nt, nullptr, n_past + t0, last);
+        if (talker_chunk(c, c->stage + (size_t) t0 * d, nt, nullptr, n_past + t0, last)) return -1;
         if (hidden_out)
             hipLaunchKernelGGL(k_rmsnorm_rows, dim3(nt), dim3(kBlock), 0, c->stream, c->xa,
                                (const float *) c->out_norm.data, g.rms_eps, d, c->hidden_all + (size_t) t0 * d);
@@ -2511,7 +2794,7 @@ int q3t_dev_talker_step(q3t_dev * c, const float * embd, int32_t n_past, float *
     if (!c || !embd) return fail(c, "step_embd is null");
     HIP_OK(hipSetDevice(c->device));
     if (check_ready(c)) return -1;
-    if (n_past < 0 || n_past + 1 > c->n_ctx) return fail(c, "Context length exceeded");
+    if (check_room(c, n_past, 1)) return -1;
     const q3t_config & g = c->cfg;
     const size_t d4 = (size_t) g.hidden_size * 4, v4 = (size_t) g.codec_vocab * 4;
     // staging layout: [FrameState | pad to 256][embd d][logits vocab][hidden d][err]
@@ -2526,7 +2809,7 @@ int q3t_dev_talker_step(q3t_dev * c, const float * embd, int32_t n_past, float *
     HIP_OK(hipMemcpyAsync(c->stage, c->pin + o_embd, d4, hipMemcpyHostToDevice, c->stream));
     bool ran = false;
     if (fk_step(c, 0, fk::MODE_TALKER_STEP, ran)) return -1;
-    if (!ran) talker_chunk(c, c->stage, 1, &c->st->talker_pos, 0, true, true);
+    if (!ran && talker_chunk(c, c->stage, 1, &c->st->talker_pos, 0, true, true)) return -1;
     if (logits_out) HIP_OK(hipMemcpyAsync(c->pin + o_logits, c->logits, v4, hipMemcpyDeviceToHost, c->stream));
     if (hidden_out) HIP_OK(hipMemcpyAsync(c->pin + o_hidden, c->hidden, d4, hipMemcpyDeviceToHost, c->stream));
     if (ran) HIP_OK(hipMemcpyAsync(c->pin + o_err, c->fk_err, 4, hipMemcpyDeviceToHost, c->stream));
@@ -2823,7 +3106,10 @@ int q3t_dev_frames_begin(q3t_dev * c, const q3t_frame_args * a) {
     if (!a->tts_pad) return fail(c, "tts_pad row is null");
     if (a->n_trailing < 0 || (a->n_trailing > 0 && !a->trailing)) return fail(c, "bad trailing rows");
     if (a->max_len < 0) return fail(c, "max_len must be >= 0");
-    if (a->n_past < 1 || a->n_past + a->max_len > c->n_ctx) return fail(c, "Context length exceeded");
+    // an 8-bit cache may be evicted between frames_run calls, which look for room themselves
+    if (a->n_past < 1 || (!c->kv_i8 && a->n_past + a->max_len > c->n_ctx)) return fail(c, "Context length exceeded");
+    if (c->kv_i8 && check_room(c, a->n_past, 0)) return -1;
+    c->frames_base = a->n_past;
     if (a->max_len > c->codes_cap) {
         dev_free(c, c->codes_out);
         c->codes_out = nullptr;
@@ -2888,6 +3174,7 @@ int q3t_dev_frames_run(q3t_dev * c, int32_t n_frames, int32_t * codes_out, int32
     if (!c->frames_ready) return fail(c, "frames_begin not called");
     HIP_OK(hipSetDevice(c->device));
     n_frames = std::max(0, std::min(n_frames, c->frames_max - c->frames_launched));
+    if (c->kv_i8 && check_room(c, c->frames_base + c->frames_launched, n_frames)) return -1;
     // Q3T_NO_GRAPH=1 enqueues the frame's kernels directly (for tracers that
     // do not follow graph launches); the kernels and results are the same.
     static const bool no_graph = [] { const char * e = std::getenv("Q3T_NO_GRAPH"); return e && e[0] == '1'; }();
@@ -2916,7 +3203,7 @@ int q3t_dev_frames_run(q3t_dev * c, int32_t n_frames, int32_t * codes_out, int32
             c->fk_refused = true;
             if (ensure_frame_graph(c)) return -1;
         }
-        if (no_graph) frame_seq(c);
+        if (no_graph) { if (frame_seq(c)) return -1; }
         else HIP_OK(hipGraphLaunch(c->frame_exec, c->stream));
         if (c->attn_layer >= 0) {
             // attention capture: a frame that emitted codes (no EOS) ran its
@@ -3329,7 +3616,7 @@ int q3t_dev_streams_reserve(q3t_dev * c, int32_t n_streams, int32_t n_ctx) {
     const q3t_config & g = c->cfg;
     if (n_streams < 1 || n_streams > 32) return fail(c, "n_streams must be in [1, 32]");
     if (n_ctx < 1) return fail(c, "n_ctx must be > 0");
-    if (c->kv_bf16) return fail(c, "multi-stream decode keeps an F16 talker cache (q3t_dev_kv_set_type F16 first)");
+    if (c->kv_bf16 || c->kv_i8) return fail(c, "multi-stream decode keeps an F16 talker cache (q3t_dev_kv_set_type F16 first)");
     bool all_q8 = true, all_f16 = true;
     for (int i = 0; i < g.n_layers + g.cp_layers; ++i) {
         const LayerDev & L = i < g.n_layers ? c->talker[i] : c->cp[i - g.n_layers];
@@ -3435,6 +3722,7 @@ namespace {
 template <class F>
 int with_stream_cache(q3t_dev * c, int32_t stream, F fn) {
     if (stream < 0 || stream >= c->nb) return fail(c, "stream index out of range (q3t_dev_streams_reserve first)");
+    if (c->kv_i8) return fail(c, "multi-stream decode keeps an F16 talker cache (q3t_dev_kv_set_type F16 first)");
     if (c->n_ctx != c->sb_ctx) return fail(c, "KV cache re-reserved since q3t_dev_streams_reserve; reserve the streams again");
     const q3t_config & g = c->cfg;
     const size_t kv = (size_t) g.n_layers * g.n_kv_head * c->sb_ctx * g.head_dim;
@@ -3632,6 +3920,7 @@ int q3t_dev_time_kernel(q3t_dev * c, int32_t which, int32_t iters, double * avg_
     GemvSpec s{};
     const int pos = std::min(c->n_ctx - 1, 512);
     if (which < 0 || which > 5) return fail(c, "unknown kernel class");
+    if (which == 4 && c->kv_i8) return fail(c, "the talker attention class needs an F16 or BF16 cache");
     if (which == 5 && !c->copy_buf) {
         // 64 MiB source + 64 MiB destination for the copy-kernel calibration
         if (dev_alloc(c, (void **) &c->copy_buf, (size_t) 2 * kCopyBytes)) return -1;

@@ -19,7 +19,7 @@ EXPORTS = [
     "q3t_dev_create", "q3t_dev_destroy", "q3t_dev_last_error", "q3t_dev_upload_tensor",
     "q3t_dev_upload_tensor_rows", "q3t_dev_staging",
     "q3t_dev_download_tensor", "q3t_dev_dequantize", "q3t_dev_kv_reserve", "q3t_dev_kv_clear",
-    "q3t_dev_kv_capacity", "q3t_dev_kv_set_type", "q3t_dev_kv_write", "q3t_dev_set_attn_capture", "q3t_dev_attn_row_count",
+    "q3t_dev_kv_capacity", "q3t_dev_kv_set_type", "q3t_dev_kv_evict", "q3t_dev_kv_read", "q3t_dev_set_rope_scaling", "q3t_dev_kv_write", "q3t_dev_set_attn_capture", "q3t_dev_attn_row_count",
     "q3t_dev_attn_row", "q3t_dev_prefill", "q3t_dev_talker_step",
     "q3t_dev_code_pred", "q3t_dev_predict_codes", "q3t_dev_stream_logits", "q3t_dev_text_proj", "q3t_dev_text_proj_noalloc", "q3t_dev_embed_rows",
     "q3t_dev_build_prefill",
@@ -69,6 +69,9 @@ def load_library(path=LIB_PATH):
         lib.q3t_dev_kv_capacity.argtypes = [vp]
         lib.q3t_dev_kv_write.argtypes = [vp, i32, i32, vp, vp]
         lib.q3t_dev_kv_set_type.argtypes = [vp, i32]
+        lib.q3t_dev_kv_evict.argtypes = [vp, i32, i32, i32, i32, vp]
+        lib.q3t_dev_kv_read.argtypes = [vp, i32, i32, i32, f32p, f32p, f32p]
+        lib.q3t_dev_set_rope_scaling.argtypes = [vp, i32, ctypes.c_double, i32, ctypes.c_float]
         lib.q3t_dev_set_attn_capture.argtypes = [vp, i32]
         lib.q3t_dev_attn_row_count.argtypes = [vp]
         lib.q3t_dev_attn_row.argtypes = [vp, i32, f32p, ctypes.c_int64, ctypes.POINTER(i32)]
@@ -183,7 +186,7 @@ class Device:
         self._check(self.lib.q3t_dev_kv_reserve(self.h, n_ctx), "kv_reserve")
 
     def kv_set_type(self, ttype):
-        """Talker cache element type for the next kv_reserve: 1 (F16) or 30 (BF16)."""
+        """Talker cache element type for the next kv_reserve: 1 (F16), 30 (BF16) or 24 (8-bit codes, I8)."""
         self._check(self.lib.q3t_dev_kv_set_type(self.h, int(ttype)), "kv_set_type")
 
     def kv_write(self, layer, k, v):
@@ -191,6 +194,23 @@ class Device:
         k = np.ascontiguousarray(k, np.uint16 if np.asarray(k).dtype == np.uint16 else np.float16)
         v = np.ascontiguousarray(v, np.uint16 if np.asarray(v).dtype == np.uint16 else np.float16)
         self._check(self.lib.q3t_dev_kv_write(self.h, layer, k.shape[0], _p(k), _p(v)), "kv_write")
+
+    def kv_evict(self, n_past, n_keep, n_sink=0, n_recent=0):
+        """I8 cache: keep n_keep slots of every layer and KV head; the kept slots [n_layers, n_kv_head, n_keep] (-1: none)."""
+        out = np.empty((self.cfg.n_layers, self.cfg.n_kv_head, max(n_keep, 0)), np.int32)
+        self._check(self.lib.q3t_dev_kv_evict(self.h, n_past, n_keep, n_sink, n_recent, _p(out)), "kv_evict")
+        return out
+
+    def kv_read(self, layer, slot0, n):
+        """I8 cache: (k, v [n, n_kv_head, head_dim], weight drawn [n_kv_head, n]) of slots slot0 .. + n."""
+        k, v = (np.empty((n, self.cfg.n_kv_head, self.cfg.head_dim), np.float32) for _ in range(2))
+        w = np.empty((self.cfg.n_kv_head, n), np.float32)
+        self._check(self.lib.q3t_dev_kv_read(self.h, layer, slot0, n, _p(k), _p(v), _p(w)), "kv_read")
+        return k, v, w
+
+    def set_rope_scaling(self, scaling, factor=1.0, n_trained=32768, mscale=1.0):
+        """I8 cache: rotary frequencies for longer contexts: 0 none, 1 linear, 2 larger base, 3 by turns."""
+        self._check(self.lib.q3t_dev_set_rope_scaling(self.h, scaling, factor, n_trained, mscale), "set_rope_scaling")
 
     # -- forward passes
     def prefill(self, embd, n_past=0, want_hidden=True):

@@ -49,9 +49,12 @@ def _rep_loop(frames, state, n_cb):
 
 def generate(dev, cfg, text, speaker=None, max_len=64, language_id=2050, repetition_penalty=1.05, temperature=0.9,
              top_k=50, instruct=None, eos_bias=0.0, target_frames=0, rep_loop_detect=False, on_frame=None, seed=0,
-             chunk=32, prefill_rows=None):
+             chunk=32, prefill_rows=None, bound=None):
     """Returns int32 codes [n_frames][n_codebooks].  `prefill_rows`, when
-    given, is (prefill, trailing, tts_pad) and skips build_prefill."""
+    given, is (prefill, trailing, tts_pad) and skips build_prefill.  `bound`
+    (n_keep, n_sink, n_recent), with an I8 cache (Device.kv_set_type(24)):
+    max_len may pass the cache; whenever the next chunk has no room the cache
+    is evicted to n_keep slots (Device.kv_evict)."""
     if max_len <= 0:
         return np.zeros((0, cfg.n_codebooks), np.int32)
     if prefill_rows is None:
@@ -59,17 +62,23 @@ def generate(dev, cfg, text, speaker=None, max_len=64, language_id=2050, repetit
     prefill, trailing, pad = prefill_rows
     plen = prefill.shape[0]
     required = plen + max_len + 8
+    if bound is not None:
+        required = min(required, max(plen, bound[0]) + chunk)
     cap = dev.lib.q3t_dev_kv_capacity(dev.h)
-    if cap < required or cap > max(required * 2, 512):
+    if cap < required or (bound is None and cap > max(required * 2, 512)):
         dev.kv_reserve(required)
+        cap = required
     dev.prefill(prefill, 0, want_hidden=False)
     dev.frames_begin(trailing, pad, plen, max_len, repetition_penalty, temperature, top_k, eos_bias, target_frames,
                      seed)
     out = []
     rep_frames, rep_state = [], {"run": 0, "start": 0}
-    produced = 0
+    produced = evicted = 0
     while produced < max_len:
         n = min(chunk, max_len - produced)
+        if bound is not None and plen + produced - evicted + n > cap:
+            dev.kv_evict(plen + produced, *bound)
+            evicted = max(evicted, plen + produced - bound[0])
         codes, eos = dev.frames_run(n)
         stop = False
         for f in range(codes.shape[0]):
