@@ -104,7 +104,6 @@ int q3t_kv8_rope(int32_t device, const q3t_kv8_rope_rows * rows, int32_t n, int6
     if (head_dim < 16 || head_dim % 16 || head_dim > 256) return refuse("head_dim must be a multiple of 16, up to 256");
     if (rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim) return refuse("rot_dim must be even, 2 to head_dim");
     kv8::RopeArgs a{};
-    int most = 1;
     for (int i = 0; i < n; ++i) {
         const q3t_kv8_rope_rows & r = rows[i];
         if (n_tokens && (!r.x || !r.y)) return refuse("null rows");
@@ -115,15 +114,15 @@ int q3t_kv8_rope(int32_t device, const q3t_kv8_rope_rows * rows, int32_t n, int6
         a.r[i] = kv8::RopeRows{r.x, r.y, r.x_token, r.x_head, r.y_token, r.y_head, r.gain, r.n_head, r.x_type, r.y_type,
                                is16(r.x) && is16(r.y) && strides16(r.x_type, {r.x_token, r.x_head}) &&
                                    strides16(r.y_type, {r.y_token, r.y_head})};
-        most = std::max(most, r.n_head);
     }
     if (!n_tokens) return 0;
     ON_DEVICE(device);
     a.pos = pos; a.pos0 = pos0; a.freq = freq; a.n_tokens = n_tokens; a.head_dim = head_dim; a.rot = rot_dim;
     a.inter = interleaved != 0; a.mscale = mscale; a.eps = eps;
-    a.per = std::min(std::max(64 / most, 1), kv8::kRopeTok);
-    hipLaunchKernelGGL(kv8::k_rope, dim3((unsigned) ((n_tokens + a.per - 1) / a.per), n), dim3(kv8::kRopeT), 0,
-                       (hipStream_t) stream, a);
+    // up to 8 tokens a workgroup, while there are two workgroups a CU
+    a.n = n;
+    a.per = (int) std::min<int64_t>(std::max<int64_t>(n_tokens / 512, 1), kv8::kRopeTok);
+    hipLaunchKernelGGL(kv8::k_rope, dim3((unsigned) ((n_tokens + a.per - 1) / a.per)), dim3(kv8::kRopeT), 0, (hipStream_t) stream, a);
     return launched("rope");
 }
 
@@ -301,8 +300,8 @@ int q3t_kv8_evict(int32_t device, const q3t_kv8 * from, const q3t_kv8 * to, cons
     ON_DEVICE(device);
     kv8::EvictArgs a{*from, *to, lens, len0, n_keep, n_sink, n_recent, kept, len_out};
     hipLaunchKernelGGL(kv8::k_evict_select, dim3(from->n_kv_head, from->n_seq), dim3(kv8::kEvT), 0, (hipStream_t) stream, a);
-    const dim3 grid((n_keep + kv8::kBlk - 1) / kv8::kBlk, from->n_kv_head, from->n_seq);
-    if (from->head_dim == 64) hipLaunchKernelGGL(kv8::k_evict_move<64>, grid, dim3(128), 0, (hipStream_t) stream, a);
+    const dim3 grid((n_keep + kv8::kMove - 1) / kv8::kMove, from->n_kv_head, from->n_seq);
+    if (from->head_dim == 64) hipLaunchKernelGGL(kv8::k_evict_move<64>, grid, dim3(256), 0, (hipStream_t) stream, a);
     else hipLaunchKernelGGL(kv8::k_evict_move<128>, grid, dim3(256), 0, (hipStream_t) stream, a);
     return launched("evict");
 }

@@ -94,7 +94,7 @@ struct RopeArgs {
     const int32_t * pos; const double * freq;
     int64_t n_tokens;
     int32_t pos0, head_dim, rot, inter;
-    int32_t per;                         // tokens a workgroup
+    int32_t per, n;                      // tokens a workgroup, tensors
     float mscale, eps;
 };
 
@@ -102,29 +102,30 @@ constexpr int kRopeT = 256;
 constexpr int kRopeMax = 128;            // pairs a row at most
 constexpr int kRopeTok = 8;              // tokens a workgroup at most
 
-// grid (tokens / per, tensors).  A workgroup takes `per` tokens of one tensor:
-// their sines and cosines first, then a row of D dims by a group of D / 16 lanes (to a
-// power of two), 16 neighbouring dims a lane; a rotated dim's partner comes through
-// LDS.
-template <int XT, int YT>
-__device__ __forceinline__ void rope_rows(const RopeArgs & a, const RopeRows & r, const float2 * cs, float * row_lds) {
-    const int D = a.head_dim, half = a.rot / 2, lanes = (D + 15) / 16;
+// Rows of `nt` tokens of one tensor: a row by a group of lanes (D / 16 of them, to a power of two), 16 dims a lane.
+// WHOLE: the lane's dims are 8 pairs (16 neighbours where interleaved, else 8 dims and the 8 half a rotation on; rot a
+// multiple of 16), so they turn in registers.  Else it has 16 neighbours, and their partners come through LDS (a
+// lane's 16 values 17 words apart, which spreads a wave's over the banks).
+template <int XT, int YT, bool WHOLE>
+__device__ __forceinline__ void rope_rows(const RopeArgs & a, const RopeRows & r, int64_t tok0, int nt, const float2 * cs,
+                                          float * row_lds) {
+    const int D = a.head_dim, half = a.rot / 2, lanes = D / 16;
     int lpr = 1;
     while (lpr < lanes) lpr <<= 1;
-    const int t = threadIdx.x, sub = t % lpr, grp = t / lpr, groups = kRopeT / lpr;
-    const int64_t tok0 = (int64_t) blockIdx.x * a.per;
-    const int nt = (int) min((int64_t) a.per, a.n_tokens - tok0), rows = nt * r.n_head;
-    float * mine = row_lds + grp * D;
-    const int d0 = sub * 16;
+    const int t = threadIdx.x, sub = t % lpr, grp = t / lpr, groups = kRopeT / lpr, rows = nt * r.n_head;
+    const bool turns = 16 * sub < a.rot;            // WHOLE: this lane's dims are rotated ones
+    const int d0 = WHOLE && !a.inter && turns ? 8 * sub : 16 * sub;
+    const int d1 = WHOLE && !a.inter && turns ? half + 8 * sub : 16 * sub + 8;
+    float * mine = row_lds + grp * 17 * lpr;
     for (int base = 0; base < rows; base += groups) {
         const int row = base + grp;
         const bool on = row < rows && sub < lanes;
         const int tok = row < rows ? row / r.n_head : 0, head = row < rows ? row % r.n_head : 0;
         float x[2][8] = {};
         if (on) {
-            const int64_t at = (tok0 + tok) * r.xt + head * r.xh + d0;
-            load8<XT>(r.x, at, r.vec, x[0]);
-            load8<XT>(r.x, at + 8, r.vec, x[1]);
+            const int64_t at = (tok0 + tok) * r.xt + head * r.xh;
+            load8<XT>(r.x, at + d0, r.vec, x[0]);
+            load8<XT>(r.x, at + d1, r.vec, x[1]);
         }
         if (r.gain) {
             float ss = 0.0f;
@@ -134,29 +135,52 @@ __device__ __forceinline__ void rope_rows(const RopeArgs & a, const RopeRows & r
             const float rs = 1.0f / sqrtf(ss / (float) D + a.eps);
             if (on)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[e / 8][e % 8] = x[e / 8][e % 8] * rs * r.gain[d0 + e];
+                for (int e = 0; e < 16; ++e) x[e / 8][e % 8] = x[e / 8][e % 8] * rs * r.gain[(e < 8 ? d0 : d1) + e % 8];
         }
-        if (on)
+        const float2 * c = cs + tok * half;
+        if constexpr (WHOLE) {
+            if (turns) {
+                c += 8 * sub;
+                if (a.inter) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) mine[d0 + e] = x[e / 8][e % 8];
-        __syncthreads();
-        if (on) {
-            const float2 * c = cs + tok * half;
+                    for (int e = 0; e < 8; ++e) {
+                        float & p = x[e / 4][2 * (e % 4)], & q = x[e / 4][2 * (e % 4) + 1];
+                        const float y = p * c[e].x - q * c[e].y;
+                        q = q * c[e].x + p * c[e].y;
+                        p = y;
+                    }
+                } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const int d = d0 + e;
-                if (d >= a.rot) continue;
-                const bool second = a.inter ? d & 1 : d >= half;
-                const int i = a.inter ? d >> 1 : second ? d - half : d;
-                const int other = a.inter ? d ^ 1 : second ? d - half : d + half;
-                const float z = x[e / 8][e % 8], w = mine[other];
-                x[e / 8][e % 8] = second ? z * c[i].x + w * c[i].y : z * c[i].x - w * c[i].y;
+                    for (int e = 0; e < 8; ++e) {
+                        const float p = x[0][e], q = x[1][e];
+                        x[0][e] = p * c[e].x - q * c[e].y;
+                        x[1][e] = q * c[e].x + p * c[e].y;
+                    }
+                }
             }
-            const int64_t at = (tok0 + tok) * r.yt + head * r.yh + d0;
-            store8<YT>(r.y, at, r.vec, x[0]);
-            store8<YT>(r.y, at + 8, r.vec, x[1]);
+        } else {
+            if (on)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mine[17 * sub + e] = x[e / 8][e % 8];
+            __syncthreads();
+            if (on)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int d = 16 * sub + e;
+                    if (d >= a.rot) continue;
+                    const bool second = a.inter ? d & 1 : d >= half;
+                    const int i = a.inter ? d >> 1 : second ? d - half : d;
+                    const int other = a.inter ? d ^ 1 : second ? d - half : d + half;
+                    const float z = x[e / 8][e % 8], y = mine[other + other / 16];
+                    x[e / 8][e % 8] = second ? z * c[i].x + y * c[i].y : z * c[i].x - y * c[i].y;
+                }
+            __syncthreads();
         }
-        __syncthreads();
+        if (on) {
+            const int64_t at = (tok0 + tok) * r.yt + head * r.yh;
+            store8<YT>(r.y, at + d0, r.vec, x[0]);
+            store8<YT>(r.y, at + d1, r.vec, x[1]);
+        }
     }
 }
 
@@ -173,10 +197,11 @@ __device__ __forceinline__ float2 rope_angle(int pos, double f, float mscale) {
     return make_float2(c * mscale, s * mscale);
 }
 
+// grid (tokens / per).  A workgroup takes `per` tokens: their sines and cosines once for all heads of all tensors, then
+// the rows.
 __global__ __launch_bounds__(kRopeT) void k_rope(RopeArgs a) {
     __shared__ float2 cs[kRopeTok * kRopeMax];
-    __shared__ float rows[kRopeT * 16];
-    const RopeRows r = a.r[blockIdx.y];
+    __shared__ float rows[kRopeT * 17];
     const int64_t tok0 = (int64_t) blockIdx.x * a.per;
     const int nt = (int) min((int64_t) a.per, a.n_tokens - tok0), half = a.rot / 2;
     for (int i = threadIdx.x; i < nt * half; i += kRopeT) {
@@ -185,9 +210,15 @@ __global__ __launch_bounds__(kRopeT) void k_rope(RopeArgs a) {
         cs[i] = rope_angle(pos, a.freq[i % half], a.mscale);
     }
     __syncthreads();
-    by_type(r.xtype, [&](auto xt) {
-        by_type(r.ytype, [&](auto yt) { rope_rows<decltype(xt)::value, decltype(yt)::value>(a, r, cs, rows); });
-    });
+    for (int x = 0; x < a.n; ++x) {
+        const RopeRows & r = a.r[x];
+        by_type(r.xtype, [&](auto xt) {
+            by_type(r.ytype, [&](auto yt) {
+                if (a.rot % 16 == 0) rope_rows<decltype(xt)::value, decltype(yt)::value, true>(a, r, tok0, nt, cs, rows);
+                else rope_rows<decltype(xt)::value, decltype(yt)::value, false>(a, r, tok0, nt, cs, rows);
+            });
+        });
+    }
 }
 
 // ------------------------------------------------------------------ append
@@ -1087,13 +1118,139 @@ __device__ __forceinline__ uint32_t order_of(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// grid (kv heads, sequences): the kept slots of one head.  The threshold (the
-// want-th largest weight of the slots between sink and recent) is found a byte at a
-// time from the top by counting; then one pass in slot order numbers the kept
-// slots, of those at the threshold the first ones.
+struct EvictLds {
+    uint32_t hist[256], cell[32 * kEvT / 64], sums[kEvT / 64], pick[2];
+};
+
+// Adds this lane's count of one to hist[bin] (on): lanes of the commonest-looking bins at once, the rest one by one, so
+// that weights of one size do not queue at one counter.
+__device__ __forceinline__ void count_bin(uint32_t * hist, uint32_t bin, bool on) {
+#pragma unroll
+    for (int x = 0; x < 3; ++x) {
+        const uint64_t left = __ballot(on);
+        if (!left) return;
+        const int first = __ffsll((unsigned long long) left) - 1;
+        const uint32_t b = __builtin_amdgcn_readlane(bin, first);
+        const uint64_t same = __ballot(on && bin == b);
+        if ((int) (threadIdx.x & 63) == first) atomicAdd(&hist[b], (uint32_t) __popcll(same));
+        on = on && bin != b;
+    }
+    if (on) atomicAdd(&hist[bin], 1u);
+}
+
+// The kept slots of one head with more than `keep` of them.  The threshold (the want-th largest weight of the slots
+// between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in slot
+// order, of those at the threshold the first ones: counts of 64 slots each by ballots, one prefix sum over them, and the
+// place of each slot by the lanes before it.  R slots a thread at a time (slot base + 1,024 r + thread): if they are all
+// there are, weights are read once.
+template <int R>
+__device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, const float * acc, int len, int32_t * kept) {
+    constexpr int kAt = R * kEvT;
+    const int t = threadIdx.x, w = t >> 6, l = t & 63;
+    const int lo = a.sink, hi = len - a.recent;     // len > keep >= sink + recent
+    const bool once = len <= kAt;
+    uint32_t key[R];
+    auto read = [&](int base) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = base + kEvT * r + t;
+            key[r] = i >= lo && i < hi ? order_of(acc[i]) : 0u;
+        }
+    };
+    if (once) read(0);
+    uint32_t want = (uint32_t) (a.keep - a.sink - a.recent), prefix = 0, mask = 0;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (t < 256) z.hist[t] = 0;
+        __syncthreads();
+        for (int base = 0; base < len; base += kAt) {
+            if (!once) read(base);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const int i = base + kEvT * r + t;
+                count_bin(z.hist, (key[r] >> shift) & 255, i >= lo && i < hi && (key[r] & mask) == prefix);
+            }
+        }
+        __syncthreads();
+        if (t < 64) {                               // the bin that the want-th largest is in, and how many are above it
+            uint32_t c[4], above = 0;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) c[x] = z.hist[255 - 4 * l - x];
+            uint32_t in = c[0] + c[1] + c[2] + c[3];
+            const uint32_t own = in;
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) {
+                const uint32_t y = __shfl_up(in, m);
+                if (l >= m) in += y;
+            }
+            above = in - own;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (above < want && above + c[x] >= want) {
+                    z.pick[0] = 255 - 4 * l - x;
+                    z.pick[1] = above;
+                }
+                above += c[x];
+            }
+        }
+        __syncthreads();
+        if (want) {                                 // 0: sink and recent slots are all
+            prefix |= z.pick[0] << shift;
+            want -= z.pick[1];
+        }
+        mask |= 255u << shift;
+        __syncthreads();
+    }
+    // prefix: the threshold; want: how many slots at it are kept
+    uint32_t over = 0, at = 0;                      // kept for sure, and at the threshold, so far
+    for (int base = 0; base < len; base += kAt) {
+        if (!once) read(base);
+        uint64_t sure[R], tie[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = base + kEvT * r + t;
+            const bool mid = i >= lo && i < hi;
+            sure[r] = __ballot(i < len && (!mid || key[r] > prefix) && (!mid || a.keep > a.sink + a.recent));
+            tie[r] = __ballot(mid && key[r] == prefix);
+            if (l == 0) z.cell[r * (kEvT / 64) + w] = (uint32_t) __popcll(sure[r]) << 16 | (uint32_t) __popcll(tie[r]);
+        }
+        __syncthreads();
+        const uint32_t own = t < R * (kEvT / 64) ? z.cell[t] : 0u;
+        uint32_t in = own;
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t y = __shfl_up(in, m);
+            if (l >= m) in += y;
+        }
+        if (l == 63) z.sums[w] = in;
+        __syncthreads();
+        uint32_t before = 0, all = 0;
+#pragma unroll
+        for (int x = 0; x < kEvT / 64; ++x) {
+            const uint32_t y = z.sums[x];
+            if (x < w) before += y;
+            all += y;
+        }
+        if (t < R * (kEvT / 64)) z.cell[t] = in + before - own;
+        __syncthreads();
+        const uint64_t lower = (1ull << l) - 1;
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = base + kEvT * r + t;
+            const uint32_t c = z.cell[r * (kEvT / 64) + w];
+            const uint32_t o = over + (c >> 16) + (uint32_t) __popcll(sure[r] & lower);
+            const uint32_t e = at + (c & 0xffffu) + (uint32_t) __popcll(tie[r] & lower);
+            if (sure[r] >> l & 1) kept[o + min(e, want)] = i;
+            else if ((tie[r] >> l & 1) && e < want) kept[o + e] = i;
+        }
+        over += all >> 16;
+        at += all & 0xffffu;
+        __syncthreads();
+    }
+}
+
+// grid (kv heads, sequences): the kept slots of one head.
 __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
-    __shared__ uint32_t hist[256], sums[kEvT / 64];
-    __shared__ uint32_t pick[2];
+    __shared__ EvictLds z;
     const int t = threadIdx.x, h = blockIdx.x, s = blockIdx.y;
     const int64_t want_len = (int64_t) (a.lens ? a.lens[s] : 0) + a.len0;
     const int len = (int) min(max(want_len, (int64_t) 0), (int64_t) a.f.n_slots), left = min(len, a.keep);
@@ -1105,92 +1262,59 @@ __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
         return;
     }
     const float * acc = a.f.acc + s * a.f.acc_seq + h * a.f.acc_head;
-    const int lo = a.sink, hi = len - a.recent;     // len > keep >= sink + recent
-    uint32_t want = (uint32_t) (a.keep - a.sink - a.recent), prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int i = lo + t; i < hi; i += kEvT) {
-            const uint32_t k = order_of(acc[i]);
-            if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (t == 0) {
-            uint32_t above = 0;
-            int b = 255;
-            while (b > 0 && above + hist[b] < want) above += hist[b--];
-            pick[0] = (uint32_t) b;
-            pick[1] = above;
-        }
-        __syncthreads();
-        prefix |= pick[0] << shift;
-        mask |= 255u << shift;
-        want -= pick[1];
-        __syncthreads();
-    }
-    // prefix: the threshold; want: how many slots at it are kept
-    uint32_t over = 0, at = 0;                      // kept for sure, and at the threshold, so far
-    for (int base = 0; base < len; base += kEvT) {
-        const int i = base + t;
-        uint32_t c = 0;
-        if (i < len) {
-            if (i < lo || i >= hi) c = 1u << 16;
-            else {
-                const uint32_t k = order_of(acc[i]);
-                c = k > prefix ? 1u << 16 : k == prefix ? 1u : 0u;
-            }
-        }
-        uint32_t in = c;                            // inclusive prefix sum of both counts (at most 1,024 each)
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const uint32_t y = __shfl_up(in, m);
-            if ((t & 63) >= m) in += y;
-        }
-        if ((t & 63) == 63) sums[t >> 6] = in;
-        __syncthreads();
-        uint32_t before = 0, all = 0;
-        for (int w = 0; w < kEvT / 64; ++w) {
-            if (w < (t >> 6)) before += sums[w];
-            all += sums[w];
-        }
-        in += before;
-        const uint32_t o = over + (in >> 16), e = at + (in & 0xffffu);      // including this slot
-        if (c >> 16) kept[o - 1 + min(e, want)] = i;
-        else if (c && e <= want) kept[o + e - 1] = i;
-        over += all >> 16;
-        at += all & 0xffffu;
-        __syncthreads();
-    }
+    if (len <= 4 * kEvT) select_slots<4>(a, z, acc, len, kept);
+    else select_slots<32>(a, z, acc, len, kept);
 }
 
-// grid (blocks of 16 kept slots, kv heads, sequences), 4 D threads: one block's
-// codes, 16 bytes a thread (K's first), scales and weights.
+constexpr int kMove = 64;                           // kept slots a workgroup of k_evict_move
+
+// grid (kept slots / 64, kv heads, sequences).  One wave looks up the slots' old places and scales, and the new scales
+// (the largest of each 16); then the codes, 16 bytes a thread at a time, all of a thread's on their way at once.
 template <int D>
-__global__ __launch_bounds__(2 * D) void k_evict_move(EvictArgs a) {
-    const int t = threadIdx.x, h = blockIdx.y, s = blockIdx.z, b = blockIdx.x;
-    const int is_v = t / D, r = t % D / (D / 16), d0 = t % (D / 16) * 16;
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+    constexpr int CH = D / 16, N = 2 * kMove * CH / 256;    // 16-byte pieces of a row; pieces a thread
+    __shared__ int32_t from[kMove];
+    __shared__ float ratio[2][kMove];
+    const int t = threadIdx.x, h = blockIdx.y, s = blockIdx.z, at = blockIdx.x * kMove;
     const int32_t * kept = a.kept + ((int64_t) s * a.f.n_kv_head + h) * a.keep;
-    const float * fs = (is_v ? a.f.vs : a.f.ks) + s * a.f.scale_seq + h * a.f.scale_head;
-    const int slot = b * kBlk + r, from = slot < a.keep ? kept[slot] : -1;
-    if (kept[b * kBlk] < 0) return;
-    const float s0 = from >= 0 ? fs[from / kBlk] : 0.0f;
-    float s1 = 0.0f;
+    const int64_t fsc = s * a.f.scale_seq + h * a.f.scale_head, tsc = s * a.t.scale_seq + h * a.t.scale_head;
+    if (t < kMove) {
+        const int slot = at + t, f = slot < a.keep ? kept[slot] : -1;
+        from[t] = f;
+        float s0[2] = {0.0f, 0.0f};
+        if (f >= 0) {
+            s0[0] = a.f.ks[fsc + f / kBlk];
+            s0[1] = a.f.vs[fsc + f / kBlk];
+            a.t.acc[s * a.t.acc_seq + h * a.t.acc_head + slot] = a.f.acc[s * a.f.acc_seq + h * a.f.acc_head + f];
+        }
 #pragma unroll
-    for (int i = 0; i < kBlk; ++i) {
-        const int o = b * kBlk + i < a.keep ? kept[b * kBlk + i] : -1;
-        if (o >= 0) s1 = fmaxf(s1, fs[o / kBlk]);
+        for (int x = 0; x < 2; ++x) {
+            float s1 = s0[x];
+#pragma unroll
+            for (int m = 1; m < kBlk; m <<= 1) s1 = fmaxf(s1, __shfl_xor(s1, m));
+            ratio[x][t] = s0[x] < s1 ? s0[x] / s1 : 1.0f;
+            if (t % kBlk == 0 && f >= 0) (x ? a.t.vs : a.t.ks)[tsc + slot / kBlk] = s1;
+        }
     }
-    if (r == 0 && d0 == 0) *((is_v ? a.t.vs : a.t.ks) + s * a.t.scale_seq + h * a.t.scale_head + b) = s1;
-    if (from < 0) return;
-    u4 w = *(const u4 *) ((is_v ? a.f.v : a.f.k) + s * a.f.seq + h * a.f.head + (int64_t) from * D + d0);
-    if (s0 < s1) {
-        const float ratio = s0 / s1;
-        const u2 p = rescale8((u2){w[0], w[1]}, ratio), q = rescale8((u2){w[2], w[3]}, ratio);
-        w = (u4){p[0], p[1], q[0], q[1]};
+    __syncthreads();
+    u4 c[N];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        const int p = x * 256 + t, row = p / CH % kMove, f = from[row];
+        const int8_t * src = (p / CH / kMove ? a.f.v : a.f.k) + s * a.f.seq + h * a.f.head + 16 * (p % CH);
+        if (f >= 0) c[x] = *(const u4 *) (src + (int64_t) f * D);
     }
-    *(u4 *) ((is_v ? a.t.v : a.t.k) + s * a.t.seq + h * a.t.head + (int64_t) slot * D + d0) = w;
-    if (!is_v && d0 == 0)
-        a.t.acc[s * a.t.acc_seq + h * a.t.acc_head + slot] = a.f.acc[s * a.f.acc_seq + h * a.f.acc_head + from];
+#pragma unroll
+    for (int x = 0; x < N; ++x) {
+        const int p = x * 256 + t, row = p / CH % kMove, is_v = p / CH / kMove;
+        if (from[row] < 0) continue;
+        const float r = ratio[is_v][row];
+        if (r != 1.0f) {
+            const u2 lo = rescale8((u2){c[x][0], c[x][1]}, r), hi = rescale8((u2){c[x][2], c[x][3]}, r);
+            c[x] = (u4){lo[0], lo[1], hi[0], hi[1]};
+        }
+        *(u4 *) ((is_v ? a.t.v : a.t.k) + s * a.t.seq + h * a.t.head + (int64_t) (at + row) * D + 16 * (p % CH)) = c[x];
+    }
 }
 
 // -------------------------------------------------------------------- read
