@@ -1119,24 +1119,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 
 struct EvictLds {
-    uint32_t hist[256], cell[32 * kEvT / 64], sums[kEvT / 64], pick[2];
+    uint32_t hist[256 * 8], total[256], cell[32 * kEvT / 64], sums[kEvT / 64], pick[2];   // hist: a copy for each lane mod 8
 };
-
-// Adds this lane's count of one to hist[bin] (on): lanes of the commonest-looking bins at once, the rest one by one, so
-// that weights of one size do not queue at one counter.
-__device__ __forceinline__ void count_bin(uint32_t * hist, uint32_t bin, bool on) {
-#pragma unroll
-    for (int x = 0; x < 3; ++x) {
-        const uint64_t left = __ballot(on);
-        if (!left) return;
-        const int first = __ffsll((unsigned long long) left) - 1;
-        const uint32_t b = __builtin_amdgcn_readlane(bin, first);
-        const uint64_t same = __ballot(on && bin == b);
-        if ((int) (threadIdx.x & 63) == first) atomicAdd(&hist[b], (uint32_t) __popcll(same));
-        on = on && bin != b;
-    }
-    if (on) atomicAdd(&hist[bin], 1u);
-}
 
 // The kept slots of one head with more than `keep` of them.  The threshold (the want-th largest weight of the slots
 // between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in slot
@@ -1160,21 +1144,26 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
     if (once) read(0);
     uint32_t want = (uint32_t) (a.keep - a.sink - a.recent), prefix = 0, mask = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
-        if (t < 256) z.hist[t] = 0;
+        for (int i = t; i < 256 * 8; i += kEvT) z.hist[i] = 0;
         __syncthreads();
         for (int base = 0; base < len; base += kAt) {
             if (!once) read(base);
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int i = base + kEvT * r + t;
-                count_bin(z.hist, (key[r] >> shift) & 255, i >= lo && i < hi && (key[r] & mask) == prefix);
-            }
+            for (int r = 0; r < R; ++r)             // key 0: no slot between sink and recent (no weight's is 0)
+                if (key[r] && (key[r] & mask) == prefix) atomicAdd(&z.hist[(key[r] >> shift & 255) * 8 + (l & 7)], 1u);
+        }
+        __syncthreads();
+        if (t < 256) {
+            uint32_t n = 0;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) n += z.hist[8 * t + x];
+            z.total[t] = n;
         }
         __syncthreads();
         if (t < 64) {                               // the bin that the want-th largest is in, and how many are above it
             uint32_t c[4], above = 0;
 #pragma unroll
-            for (int x = 0; x < 4; ++x) c[x] = z.hist[255 - 4 * l - x];
+            for (int x = 0; x < 4; ++x) c[x] = z.total[255 - 4 * l - x];
             uint32_t in = c[0] + c[1] + c[2] + c[3];
             const uint32_t own = in;
 #pragma unroll
@@ -1204,14 +1193,17 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
     uint32_t over = 0, at = 0;                      // kept for sure, and at the threshold, so far
     for (int base = 0; base < len; base += kAt) {
         if (!once) read(base);
-        uint64_t sure[R], tie[R];
+        // of those between sink and recent, the ones above the threshold; none where sink and recent are all
+        const uint32_t least = a.keep > a.sink + a.recent ? prefix : 0xffffffffu;
+        auto sure = [&](int r) {
+            const int i = base + kEvT * r + t;
+            return key[r] ? key[r] > least : i < len;
+        };
+        auto tie = [&](int r) { return key[r] && key[r] == prefix; };
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int i = base + kEvT * r + t;
-            const bool mid = i >= lo && i < hi;
-            sure[r] = __ballot(i < len && (!mid || key[r] > prefix) && (!mid || a.keep > a.sink + a.recent));
-            tie[r] = __ballot(mid && key[r] == prefix);
-            if (l == 0) z.cell[r * (kEvT / 64) + w] = (uint32_t) __popcll(sure[r]) << 16 | (uint32_t) __popcll(tie[r]);
+            const uint64_t s = __ballot(sure(r)), e = __ballot(tie(r));
+            if (l == 0) z.cell[r * (kEvT / 64) + w] = (uint32_t) __popcll(s) << 16 | (uint32_t) __popcll(e);
         }
         __syncthreads();
         const uint32_t own = t < R * (kEvT / 64) ? z.cell[t] : 0u;
@@ -1232,15 +1224,15 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
         }
         if (t < R * (kEvT / 64)) z.cell[t] = in + before - own;
         __syncthreads();
-        const uint64_t lower = (1ull << l) - 1;
+        auto lanes_before = [](uint64_t m) {
+            return __builtin_amdgcn_mbcnt_hi((uint32_t) (m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t) m, 0u));
+        };
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-            const int i = base + kEvT * r + t;
+            const bool is = sure(r), ie = tie(r);
             const uint32_t c = z.cell[r * (kEvT / 64) + w];
-            const uint32_t o = over + (c >> 16) + (uint32_t) __popcll(sure[r] & lower);
-            const uint32_t e = at + (c & 0xffffu) + (uint32_t) __popcll(tie[r] & lower);
-            if (sure[r] >> l & 1) kept[o + min(e, want)] = i;
-            else if ((tie[r] >> l & 1) && e < want) kept[o + e] = i;
+            const uint32_t o = over + (c >> 16) + lanes_before(__ballot(is)), e = at + (c & 0xffffu) + lanes_before(__ballot(ie));
+            if (is || (ie && e < want)) kept[o + min(e, want)] = base + kEvT * r + t;
         }
         over += all >> 16;
         at += all & 0xffffu;
