@@ -9,6 +9,7 @@ device and torch's current stream there, and return without waiting; lengths
 and positions are int32 tensors on that device.
 """
 import ctypes
+import struct
 
 import numpy as np
 import torch
@@ -48,6 +49,20 @@ class CAttendArgs(ctypes.Structure):
                 ("scale", _f32), ("weights", _i32)]
 
 
+def _packer(cls):
+    """A struct.Struct with the fields of a ctypes structure at their places (filling one of these is a call's
+    largest host cost otherwise)."""
+    code, at = "", 0
+    for name, kind in cls._fields_:
+        f = getattr(cls, name)
+        code += "%dx" % (f.offset - at) if f.offset > at else ""
+        code += {_vp: "Q", _i64: "q", _i32: "i", _f32: "f"}[kind]
+        at = f.offset + f.size
+    return struct.Struct("=" + code + ("%dx" % (ctypes.sizeof(cls) - at) if ctypes.sizeof(cls) > at else ""))
+
+
+_pack_rope, _pack_attend = _packer(CRopeRows).pack, _packer(CAttendArgs).pack
+
 _lib = None
 
 
@@ -60,12 +75,12 @@ def load_kv8_library():
         lib.q3t_kv8_last_error.argtypes = []
         lib.q3t_kv8_last_error.restype = ctypes.c_char_p
         lib.q3t_kv8_rope_freqs.argtypes = [_i32, ctypes.c_double, _i32, ctypes.c_double, _i32, _vp]
-        lib.q3t_kv8_rope.argtypes = [_i32, ctypes.POINTER(CRopeRows), _i32, _i64, _i32, _i32, _i32, _vp, _i32, _vp,
+        lib.q3t_kv8_rope.argtypes = [_i32, _vp, _i32, _i64, _i32, _i32, _i32, _vp, _i32, _vp,
                                      _f32, _f32, _vp]
         lib.q3t_kv8_append.argtypes = [_i32, cc, _vp, _vp, _i32, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _vp]
-        lib.q3t_kv8_attend_ws.argtypes = [cc, ctypes.POINTER(CAttendArgs)]
+        lib.q3t_kv8_attend_ws.argtypes = [cc, _vp]
         lib.q3t_kv8_attend_ws.restype = _i64
-        lib.q3t_kv8_attend.argtypes = [_i32, cc, ctypes.POINTER(CAttendArgs), _vp, _i64, _vp]
+        lib.q3t_kv8_attend.argtypes = [_i32, cc, _vp, _vp, _i64, _vp]
         lib.q3t_kv8_evict.argtypes = [_i32, cc, cc, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp]
         lib.q3t_kv8_read.argtypes = [_i32, cc, _vp, _i32, _i32, _i32, _vp, _vp, _vp]
         _lib = lib
@@ -87,17 +102,21 @@ def _need(ok, message):
         raise Kv8Error(message)
 
 
-def _ints(t, n, device, what):
-    """Address of an int32 device tensor of n values (0 for None)."""
+def _ints(t, n, index, what):
+    """Address of an int32 tensor of n values on GPU `index` (0 for None)."""
     if t is None:
         return 0
-    _need(t.dtype == torch.int32 and t.device == device and t.shape == (n,) and t.is_contiguous(),
-          f"{what} must be {n} contiguous int32 on {device}")
+    if t.dtype is not torch.int32 or t.get_device() != index or t.shape != (n,) or not t.is_contiguous():
+        raise Kv8Error(f"{what} must be {n} contiguous int32 on the same GPU")
     return t.data_ptr()
 
 
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _stream(index):
+    """torch's current stream on GPU `index`"""
+    return _raw_stream(index) if _raw_stream else torch.cuda.current_stream(index).cuda_stream
 
 
 class Cache:
@@ -117,7 +136,7 @@ class Cache:
             _need(acc.dtype == torch.float32 and acc.shape == (s, h, c) and acc.device == k.device and acc.stride(2) == 1,
                   "acc must be float32 [S, H, C] with dense slots")
         self.tensors = (k, v, ks, vs, acc)      # keeps the memory alive
-        self.device, self.shape = k.device, (s, h, c, d)
+        self.device, self.index, self.shape = k.device, k.get_device(), (s, h, c, d)
         self.c = CCache(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), None if acc is None else acc.data_ptr(),
                         k.stride(0), k.stride(1), ks.stride(0), ks.stride(1), 0 if acc is None else acc.stride(0),
                         0 if acc is None else acc.stride(1), s, h, c, d)
@@ -146,30 +165,30 @@ def rope(xs, pos, freq, *, gains=None, outs=None, dtype=None, interleaved=False,
     """Rotates the first 2 * len(freq) dims of the rows of each tensor [T, heads, D] in xs (one to four, one launch) by
     pos [T] (int32), after an RMS norm with that tensor's gain where it has one.  outs: tensors to write (x itself: in
     place); without, new ones in `dtype` (default x's).  Returns the outputs."""
-    x0 = xs[0]
-    device, (t, _, d) = x0.device, x0.shape
-    _need(freq.dtype == torch.float64 and freq.device == device and freq.dim() == 1 and freq.is_contiguous(),
-          "freq must be contiguous float64 on the rows' device")
-    gains = gains or [None] * len(xs)
+    n = len(xs)
+    gains = gains or [None] * n
     if outs is None:
-        outs = [torch.empty(x.shape, dtype=dtype or x.dtype, device=device) for x in xs]
-    _need(1 <= len(xs) <= 4 and len(gains) == len(xs) and len(outs) == len(xs), "1 to 4 tensors, as many gains and outputs")
-    rows = (CRopeRows * len(xs))()
-    for r, x, y, g in zip(rows, xs, outs, gains):
-        _need(x.dim() == 3 and x.shape[0] == t and x.shape[2] == d and y.shape == x.shape and x.device == device and
-              y.device == device and x.is_cuda, "rows must be [T, heads, D] on one GPU, outputs of the same shape")
-        _need(x.dtype in _TYPES and y.dtype in _TYPES, "rows must be float32, float16 or bfloat16")
-        _need((x.stride(2) == 1 and y.stride(2) == 1) or x.numel() == 0, "rows' dims must be dense")
-        if g is not None:
-            _need(g.dtype == torch.float32 and g.shape == (d,) and g.device == device and g.is_contiguous(),
-                  "a gain must be contiguous float32 [D]")
-        r.x, r.y, r.gain = x.data_ptr(), y.data_ptr(), None if g is None else g.data_ptr()
-        r.x_token, r.x_head, _ = x.stride()
-        r.y_token, r.y_head, _ = y.stride()
-        r.n_head, r.x_type, r.y_type = x.shape[1], _TYPES[x.dtype], _TYPES[y.dtype]
-    _check(load_kv8_library().q3t_kv8_rope(device.index, rows, len(xs), t, d, 2 * freq.numel(), bool(interleaved),
-                                           _ints(pos, t, device, "pos"), 0, freq.data_ptr(), mscale, eps,
-                                           _stream(device)), "rope")
+        outs = [torch.empty_like(x, dtype=dtype, memory_format=torch.contiguous_format) for x in xs]
+    _need(1 <= n <= 4 and len(gains) == n and len(outs) == n, "1 to 4 tensors, as many gains and outputs")
+    index = xs[0].get_device()
+    t, d = xs[0].shape[0], xs[0].shape[-1]
+    if freq.dtype is not torch.float64 or freq.get_device() != index or freq.dim() != 1 or not freq.is_contiguous():
+        raise Kv8Error("freq must be contiguous float64 on the rows' GPU")
+    rows = b""
+    for x, y, g in zip(xs, outs, gains):
+        shape = x.shape
+        if len(shape) != 3 or shape[0] != t or shape[2] != d or y.shape != shape or index < 0 or x.get_device() != index or \
+                y.get_device() != index:
+            raise Kv8Error("rows must be [T, heads, D] on one GPU, outputs of the same shape")
+        xt, yt, (xa, xb, xc), (ya, yb, yc) = _TYPES.get(x.dtype), _TYPES.get(y.dtype), x.stride(), y.stride()
+        _need(xt is not None and yt is not None, "rows must be float32, float16 or bfloat16")
+        _need((xc == 1 and yc == 1) or t == 0, "rows' dims must be dense")
+        if g is not None and (g.dtype is not torch.float32 or g.shape != (d,) or g.get_device() != index or not g.is_contiguous()):
+            raise Kv8Error("a gain must be contiguous float32 [D]")
+        rows += _pack_rope(x.data_ptr(), y.data_ptr(), xa, xb, ya, yb, 0 if g is None else g.data_ptr(), shape[1], xt, yt)
+    _check((_lib or load_kv8_library()).q3t_kv8_rope(index, rows, n, t, d, 2 * freq.shape[0], bool(interleaved),
+                                                     _ints(pos, t, index, "pos"), 0, freq.data_ptr(), mscale, eps,
+                                                     _stream(index)), "rope")
     return outs
 
 
@@ -177,15 +196,16 @@ def append(cache, k, v, start, n_new=None):
     """Stores rows k, v [S, n, H, D] (float32, float16 or bfloat16, alike) from slot start[s] on; n_new [S]: how many of
     a sequence's rows are rows (the rest is padding)."""
     s, h, _, d = cache.shape
-    _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.stride() == v.stride() and
-          k.device == cache.device and v.device == cache.device and (k.stride(3) == 1 or k.numel() == 0),
-          "rows must be [S, n, H, D], k and v alike, with dense dims")
-    _need(k.shape[0] == s and k.shape[2:] == (h, d), f"rows must be [{s}, n, {h}, {d}]")
-    _need(k.dtype in _TYPES, "rows must be float32, float16 or bfloat16")
-    _check(load_kv8_library().q3t_kv8_append(cache.device.index, cache.ref, k.data_ptr(), v.data_ptr(), _TYPES[k.dtype],
-                                             k.stride(0), k.stride(1), k.stride(2), k.shape[1],
-                                             _ints(start, s, cache.device, "start"), 0,
-                                             _ints(n_new, s, cache.device, "n_new"), _stream(cache.device)), "append")
+    index, shape, stride, t = cache.index, k.shape, k.stride(), _TYPES.get(k.dtype)
+    if len(shape) != 4 or shape[0] != s or shape[2] != h or shape[3] != d:
+        raise Kv8Error(f"rows must be [{s}, n, {h}, {d}]")
+    if shape != v.shape or k.dtype is not v.dtype or stride != v.stride() or k.get_device() != index or \
+            v.get_device() != index or (stride[3] != 1 and shape[1]):
+        raise Kv8Error("rows k and v must be alike, with dense dims, on the cache's GPU")
+    _need(t is not None, "rows must be float32, float16 or bfloat16")
+    _check((_lib or load_kv8_library()).q3t_kv8_append(index, cache.ref, k.data_ptr(), v.data_ptr(), t, stride[0], stride[1],
+                                                       stride[2], shape[1], _ints(start, s, index, "start"), 0,
+                                                       _ints(n_new, s, index, "n_new"), _stream(index)), "append")
 
 
 def attend(cache, q, lens, *, scale=None, n_new=None, causal=True, weights=False, max_len=0, out=None, dtype=None):
@@ -194,24 +214,24 @@ def attend(cache, q, lens, *, scale=None, n_new=None, causal=True, weights=False
     slot drew.  max_len: the longest sequence to size the call for (default: all slots).  out: where to write
     (default: a new tensor of `dtype`, by default q's); rows past n_new are left as they were."""
     s, h, _, d = cache.shape
-    device = cache.device
-    _need(q.dim() == 4 and q.shape[0] == s and q.shape[3] == d and q.device == device and
-          (q.stride(3) == 1 or q.numel() == 0), f"q must be [{s}, n, heads, {d}] with dense dims")
+    index, shape, stride = cache.index, q.shape, q.stride()
+    if len(shape) != 4 or shape[0] != s or shape[3] != d or q.get_device() != index or (stride[3] != 1 and shape[1]):
+        raise Kv8Error(f"q must be [{s}, n, heads, {d}] with dense dims, on the cache's GPU")
     if out is None:
-        out = torch.empty(q.shape, dtype=dtype or q.dtype, device=device)
-    _need(out.shape == q.shape and out.device == device and (out.stride(3) == 1 or q.numel() == 0),
-          "out must have q's shape, with dense dims")
-    _need(q.dtype in _TYPES and out.dtype in _TYPES, "q must be float16 or bfloat16, out one of these or float32")
-    a = CAttendArgs(q.data_ptr(), out.data_ptr(), *q.stride()[:3], *out.stride()[:3], _TYPES[q.dtype], _TYPES[out.dtype],
-                    q.shape[1], q.shape[2], _ints(lens, s, device, "lens"), 0, _ints(n_new, s, device, "n_new"),
-                    max_len, causal, d ** -0.5 if scale is None else scale, weights)
-    lib = load_kv8_library()
-    ref = ctypes.byref(a)
-    need = _check(lib.q3t_kv8_attend_ws(cache.ref, ref), "attend")
+        out = torch.empty_like(q, dtype=dtype, memory_format=torch.contiguous_format)
+    ostride = out.stride()
+    if out.shape != shape or out.get_device() != index or (ostride[3] != 1 and shape[1]):
+        raise Kv8Error("out must have q's shape, with dense dims, on its GPU")
+    qt, ot = _TYPES.get(q.dtype), _TYPES.get(out.dtype)
+    _need(qt is not None and ot is not None, "q must be float16 or bfloat16, out one of these or float32")
+    args = _pack_attend(q.data_ptr(), out.data_ptr(), stride[0], stride[1], stride[2], ostride[0], ostride[1], ostride[2],
+                        qt, ot, shape[1], shape[2], _ints(lens, s, index, "lens"), 0, _ints(n_new, s, index, "n_new"),
+                        max_len, bool(causal), d ** -0.5 if scale is None else scale, bool(weights))
+    lib = _lib or load_kv8_library()
+    need = _check(lib.q3t_kv8_attend_ws(cache.ref, args), "attend")
     # from torch's allocator on the current stream: reused only behind this call's kernels, and a captured graph's own
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    _check(lib.q3t_kv8_attend(device.index, cache.ref, ref, ws.data_ptr() if need else None, need, _stream(device)),
-           "attend")
+    ws = torch.empty(need, dtype=torch.uint8, device=cache.device) if need else None
+    _check(lib.q3t_kv8_attend(index, cache.ref, args, ws.data_ptr() if need else None, need, _stream(index)), "attend")
     return out
 
 
@@ -220,21 +240,22 @@ def evict(cache, to, lens, *, n_keep, n_sink=0, n_recent=0):
     their order: the first n_sink, the last n_recent, and of the rest those that drew the most weight.  Returns (kept
     [S, H, n_keep] int32: the old slots, -1 behind them; the new lengths [S] int32)."""
     s, h = cache.shape[:2]
-    device = cache.device
-    _need(to.device == device, "both caches must be on one device")
+    index = cache.index
+    _need(to.index == index, "both caches must be on one GPU")
     _need(n_keep >= 1, "n_keep must be at least 1")
-    kept = torch.empty(s, h, n_keep, dtype=torch.int32, device=device)
-    left = torch.empty(s, dtype=torch.int32, device=device)
-    _check(load_kv8_library().q3t_kv8_evict(device.index, cache.ref, to.ref, _ints(lens, s, device, "lens"), 0, n_keep,
-                                            n_sink, n_recent, kept.data_ptr(), left.data_ptr(), _stream(device)), "evict")
+    kept = torch.empty(s, h, n_keep, dtype=torch.int32, device=cache.device)
+    left = torch.empty(s, dtype=torch.int32, device=cache.device)
+    _check((_lib or load_kv8_library()).q3t_kv8_evict(index, cache.ref, to.ref, _ints(lens, s, index, "lens"), 0, n_keep, n_sink,
+                                                      n_recent, kept.data_ptr(), left.data_ptr(), _stream(index)), "evict")
     return kept, left
 
 
 def read(cache, start, n, *, dtype=torch.float32):
     """Values of slots start[s] .. + n of every head: (k, v), each [S, n, H, D] in `dtype`; 0 outside the cache."""
     s, h, _, d = cache.shape
+    index = cache.index
     _need(dtype in _TYPES and n >= 0, "dtype must be float32, float16 or bfloat16, n not negative")
     k, v = (torch.empty(s, n, h, d, dtype=dtype, device=cache.device) for _ in range(2))
-    _check(load_kv8_library().q3t_kv8_read(cache.device.index, cache.ref, _ints(start, s, cache.device, "start"), 0, n,
-                                           _TYPES[dtype], k.data_ptr(), v.data_ptr(), _stream(cache.device)), "read")
+    _check((_lib or load_kv8_library()).q3t_kv8_read(index, cache.ref, _ints(start, s, index, "start"), 0, n, _TYPES[dtype],
+                                                     k.data_ptr(), v.data_ptr(), _stream(index)), "read")
     return k, v
