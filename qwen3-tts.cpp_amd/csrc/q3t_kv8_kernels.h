@@ -800,23 +800,6 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
     if (split && t0 >= t1) return;
     const bool work = row0 + 16 * RT * w < rows;        // this wave has rows
 
-    h8v q[RT][NC];
-    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
-    int lim[RT];
-    f4 o[RT][NJ];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-        const int row = row0 + 16 * (RT * w + r) + i;
-        const bool on = row < rows;
-        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, 64, q[r]);
-        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, 64, q[r], qs[r]);
-        lim[r] = on ? row_limit(a, len, n, tok) : 0;
-        m[r] = -INFINITY;
-        sum[r] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
-    }
     const int plain = row_limit(a, len, n, row0 / a.group) / 64;    // tiles before this one need no mask
     const int last = len - 1, last_blk = last / kBlk;
 
@@ -872,6 +855,27 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
         for (int j = 0; j < 4; ++j)
             *(u4 *) (d + j * 64 + ((vc ^ (vq & 7) ^ (2 * j)) << 3)) = (u4){f[j][0], f[j][1], f[j][2], f[j][3]};
     };
+    if (t0 < t1) {
+        fetch_k(t0);
+        fetch_v(t0);
+    }
+    h8v q[RT][NC];
+    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
+    int lim[RT];
+    f4 o[RT][NJ];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = row0 + 16 * (RT * w + r) + i;
+        const bool on = row < rows;
+        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
+        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, 64, q[r]);
+        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, 64, q[r], qs[r]);
+        lim[r] = on ? row_limit(a, len, n, tok) : 0;
+        m[r] = -INFINITY;
+        sum[r] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
+    }
     auto step = [&](int tile, auto masked) {
         const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
         fetch_k(tile + 1);
@@ -983,8 +987,6 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
         __syncthreads();
     };
     if (t0 < t1) {
-        fetch_k(t0);
-        fetch_v(t0);
         stash_k(t0);
         stash_v(t0);
         __syncthreads();
@@ -1019,74 +1021,86 @@ __global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
     }
 }
 
-// acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels left.
-// Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that none
-// is above its row's maximum; K in registers; the sum over rows is one over lanes i, in order of the row tiles.
-// by_rows: grid (slot tiles, kv heads, sequences), the four waves take the row tiles in turn and add up; else a wave takes a slot tile.
+// acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels
+// left.  Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that none
+// is above its row's maximum; K in registers, the next 16 rows on their way while these are worked on; the sum over rows
+// is one over lanes i, in order of the row tiles.  Bound by the vector ALU (an exponential a score) and, at 3 waves a
+// SIMD, by its last turn; 128 slots a wave would need half the row reads, but one wave a SIMD: 100 us where this takes 55.
+// grid (slot tiles / 4 * by, kv heads, sequences): `by` (1, 2 or 4) waves take the row tiles of one slot tile in turn and
+// add up in their order.
 template <int D>
-__global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows, int lo) {
-    constexpr int NC = D / 32;
+__global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int lo) {
+    constexpr int NC = D / 32, NB = 4;
     __shared__ float part[4][64];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
     const int heads = a.c.n_kv_head, g = blockIdx.y, s = blockIdx.z;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
-    const int tile = by_rows ? blockIdx.x : 4 * blockIdx.x + w, j0 = tile * 64;
+    const int j0 = (blockIdx.x * (4 / by) + w / by) * 64;
     const int64_t hd = (int64_t) s * heads + g;
-    float add[4][4] = {};
+    float add[NB][4] = {};
     if (j0 < len && n) {
-        const int last = len - 1, last_blk = last / kBlk;
-        h8v kf[4][NC];
-        float ks[4];
+        const int last = len - 1;
+        h8v kf[NB][NC];
+        float ks[NB];
         const int off = lo == 8 ? 16 * k : 8 * k;
         const int8_t * kb = a.c.k + s * a.c.seq + g * a.c.head + off;
+        const float * sb = a.c.ks + s * a.c.scale_seq + g * a.c.scale_head;
 #pragma unroll
-        for (int b = 0; b < 4; ++b) {
+        for (int b = 0; b < NB; ++b) {
             const int8_t * p = kb + (int64_t) min(j0 + 16 * b + i, last) * D;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 const u2 x = *(const u2 *) (p + lo * (c & 1) + 64 * (c >> 1));
                 kf[b][c] = halves8(x[0], x[1]);
             }
-            ks[b] = (a.c.ks + s * a.c.scale_seq + g * a.c.scale_head)[min(tile * 4 + b, last_blk)];
+            ks[b] = sb[min(j0 + 16 * b, last) / kBlk];
         }
         // the first row that sees slot j0
-        const int rt0 = (a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0) + (by_rows ? w : 0), rt1 = (rows + 15) / 16;
-        const int stride = by_rows ? 4 : 1;
+        const int rt0 = (a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0) + w % by, rt1 = (rows + 15) / 16;
+        // from this row on a row sees all of these slots: none is masked (a row past the last one has a finite row's scores)
+        const int clear = a.causal ? max(j0 + 63 - (len - n), 0) * a.group : 0;
+        const uint16_t * qb = a.qh + hd * a.rows16 * D;
+        const f4 * rb = a.rowq + hd * a.rows16;
         h8v q[NC];
         f4 rq;
         auto fetch = [&](int rt) {
-            const int64_t at = hd * a.rows16 + min(16 * min(rt, rt1 - 1) + i, rows - 1);
+            const uint32_t at = (uint32_t) min(16 * rt + i, rows - 1);
 #pragma unroll
-            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (a.qh + at * D + off + lo * (c & 1) + 64 * (c >> 1));
-            rq = a.rowq[at];
+            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (qb + (at * D + (uint32_t) (off + lo * (c & 1) + 64 * (c >> 1))));
+            rq = rb[at];
         };
         if (rt0 < rt1) fetch(rt0);
-        for (int rt = rt0; rt < rt1; rt += stride) {
+        for (int rt = rt0; rt < rt1; rt += by) {
             const int row = 16 * rt + i;
-            f4 sc[4];
+            f4 sc[NB];
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int b = 0; b < 4; ++b) sc[b] = mfma32(kf[b][c], q[c], c ? sc[b] : (f4){0.f, 0.f, 0.f, 0.f});
+                for (int b = 0; b < NB; ++b) sc[b] = mfma32(kf[b][c], q[c], c ? sc[b] : (f4){0.f, 0.f, 0.f, 0.f});
             const float factor = rq[0], top = rq[1], inv = row < rows ? rq[2] : 0.0f;
-            fetch(rt + stride);
-            // rows that see all of these slots: none is masked (a row past the last one has a finite row's scores)
-            const bool all = row_limit(a, len, n, 16 * rt / a.group) >= j0 + 64;
-            const int lim = row_limit(a, len, n, min(row, rows - 1) / a.group);
+            fetch(rt + by);
+            if (16 * rt < clear) {
+                const int lim = row_limit(a, len, n, min(row, rows - 1) / a.group);
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(sc[b][e] * (ks[b] * factor) - top);
+                        add[b][e] = fmaf(j0 + 16 * b + 4 * k + e < lim ? x : 0.0f, inv, add[b][e]);
+                    }
+                continue;
+            }
+#pragma unroll
+            for (int b = 0; b < NB; ++b) {
                 const float f = ks[b] * factor;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = __builtin_amdgcn_exp2f(sc[b][e] * f - top);
-                    if (!all) x = j0 + 16 * b + 4 * k + e < lim ? x : 0.0f;
-                    add[b][e] = fmaf(x, inv, add[b][e]);
-                }
+                for (int e = 0; e < 4; ++e)
+                    add[b][e] = fmaf(__builtin_amdgcn_exp2f(sc[b][e] * f - top), inv, add[b][e]);
             }
         }
     }
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -1094,11 +1108,11 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by_rows,
             if (i == 0) part[w][16 * b + 4 * k + e] = add[b][e];
         }
     __syncthreads();
-    if (by_rows && w) return;
     const int j = j0 + l;
-    if (j >= len || !n) return;
-    a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] +=
-        by_rows ? ((part[0][l] + part[1][l]) + part[2][l]) + part[3][l] : part[w][l];
+    if (w % by || !n || j >= len) return;
+    float sum = part[w][l];
+    for (int y = 1; y < by; ++y) sum += part[w + y][l];
+    a.c.acc[s * a.c.acc_seq + g * a.c.acc_head + j] += sum;
 }
 
 // ---------------------------------------------------------------- eviction
