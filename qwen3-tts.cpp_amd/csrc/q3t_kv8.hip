@@ -230,7 +230,7 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
         if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1>), grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((kv8::k_attend_few<D, 2>), grid, dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL((kv8::k_attend_tile<D, 2>), dim3(H * S, p.row_tiles, p.n_split), dim3(kv8::kTileT), 0, st, a);
+        hipLaunchKernelGGL(kv8::k_attend_tile<D>, dim3(H * S, p.row_tiles, p.n_split), dim3(kv8::kTileT), 0, st, a);
     }
     const bool many = p.n_split > 8;
     a.row_blocks = p.n_split == 1 ? 0 : many ? rows : (rows + 1024 / D - 1) / (1024 / D);

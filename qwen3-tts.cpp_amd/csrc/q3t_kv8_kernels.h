@@ -773,9 +773,9 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 }
 
 // ----------------------------------------------- attention of many rows
-// A tile of 64 RT rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
+// A tile of 128 rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
 // fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four waves of
-// 16 RT rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
+// 32 rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
 // k_attend_few; here all waves go through the same tiles, with dims in their own order:
 //   K in LDS: [slot][dim] in 16-byte chunks, chunk c of slot t at c ^ (t % (D / 8));
 //   V in LDS: [dim][8 chunks], chunk 4u + k = slots 32u + 4k + e, then 32u + 16 + 4k + e (an operand of the
@@ -784,17 +784,17 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 // Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to LDS
 // at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the MFMAs of
 // these: left to itself the compiler waits for each read alone.
-template <int D, int RT>
-__global__ __launch_bounds__(256, 2) void k_attend_tile(AttendArgs a) {
-    constexpr int NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
+template <int D>
+__global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
+    constexpr int RT = 2, NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
     __shared__ __align__(16) uint16_t lds[4 * KT];      // K of even and odd tiles, V of even and odd tiles
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
     const int heads = a.c.n_kv_head, s = blockIdx.x / heads, g = blockIdx.x % heads;
     const int row_tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
-    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, row0 = row_tile * 64 * RT;
+    const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, row0 = row_tile * kTileRows;
     if (row0 >= rows) return;
     const int64_t hd = (int64_t) s * heads + g;
-    const int lim_top = row_limit(a, len, n, (min(row0 + 64 * RT, rows) - 1) / a.group);
+    const int lim_top = row_limit(a, len, n, (min(row0 + kTileRows, rows) - 1) / a.group);
     const int t0 = split * a.split_tiles, t1 = min(t0 + a.split_tiles, (lim_top + 63) / 64);
     const bool parts = splits_of(a, lim_top) > 1;
     if (split && t0 >= t1) return;

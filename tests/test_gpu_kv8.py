@@ -426,6 +426,15 @@ def test_attend_long():
         check_attend(c, query(1, n, 16, 64, g, torch.float16, 2.0), [40001])
 
 
+@pytest.mark.parametrize("s,h,slots", [(1, 1, 700), (3, 8, 4001), (5, 8, 2500), (2, 5, 13000)])
+def test_attend_many_rows_of_many_sizes(s, h, slots):
+    """60 rows of two heads over few and many slot tiles: how many waves share a tile of the weights' pass, and into how many
+    splits the slots go, changes with the size."""
+    g = gen(slots)
+    c = fill(s, h, -(-slots // 16) * 16, 128, g, spread=0.3)
+    check_attend(c, query(s, 60, 2 * h, 128, g, torch.float16, 1.5), [slots - 37 * b for b in range(s)])
+
+
 def test_attend_offsets_past_32_bits():
     """A head whose codes lie past 2^31 bytes, at slots past 2^31 bytes of it."""
     c = kv8.empty(1, 2, 17_000_000, 128)
