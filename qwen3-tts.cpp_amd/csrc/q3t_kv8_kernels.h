@@ -1,5 +1,7 @@
 // q3t_kv8_kernels.h -- kernels of the 8-bit attention cache's operators
 // (include/q3t_kv8.h): rotary positions, append, attention, eviction, read.
+// Times are one MI355X's, kernels alone; a large copy runs at 5.2 TB/s there
+// and an 8192^3 fp16 library product at 1,160 TFLOP/s.
 #pragma once
 
 #include "../../include/q3t_kv8.h"
@@ -197,6 +199,8 @@ __device__ __forceinline__ float2 rope_angle(int pos, double f, float mscale) {
     return make_float2(c * mscale, s * mscale);
 }
 
+// Bound by memory: 11,301 tokens of 36 heads (208 MB) 39 us, 2,049 tokens of 24 heads from fp32 to fp16 (38 MB) 10 us,
+// one token 4.8 us.  All rows through LDS took 106, 20 and 5.6: words 16 apart in the banks, and the angles once a tensor.
 // grid (tokens / per).  A workgroup takes `per` tokens: their sines and cosines once for all heads of all tensors, then
 // the rows.
 __global__ __launch_bounds__(kRopeT) void k_rope(RopeArgs a) {
@@ -255,7 +259,9 @@ __device__ __forceinline__ u2 rescale8(u2 w, float r) {
 }
 
 // grid (blocks a sequence's rows can touch, heads * 2, sequences); 2 D threads:
-// one workgroup a block of 16 slots and K or V, 8 dims of a row a thread.
+// one workgroup a block of 16 slots and K or V, 8 dims of a row a thread, so that a block's maximum, the codes it
+// held before and its new ones meet in one place and a block has one writer.  Bound by its chain of one load, the
+// maximum over the block and the divisions: 2,049 rows of 8 heads (12.6 MB) 7.7 us, one row of 16 sequences 3.6.
 template <int D, int T>
 __global__ __launch_bounds__(2 * D) void k_append(AppendArgs a) {
     __shared__ float part[2 * D / 64];
@@ -442,12 +448,19 @@ __device__ __forceinline__ float max_rows(float x) {
 // A row's base of exponents follows its largest score only once that is more than this above it: a tile then needs
 // no exchange between lanes and no rescaling as a rule, and 2^1.9 kPScale is still an fp16 number.
 constexpr float kSlack = 1.9f;
+// The largest value scale of blocks b0 .. b1 - 1 (all 64 lanes).
+__device__ __forceinline__ float top_scale(const float * vs, int b0, int b1, int lane) {
+    float x = 0.0f;
+    for (int b = b0 + lane; b < b1; b += 64) x = fmaxf(x, vs[b]);
+    return wave_max_f(x);
+}
 constexpr float kPScale = 16384.0f;    // probabilities enter the value product times this (fp16's normal range then ends at 2^-28)
 
 // Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), four
 // waves; workgroups go to the XCDs in turn, so heads come first and a sequence's splits are turned by its number: the
-// first splits, the only ones of short sequences, spread over all XCDs.  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its own running
-// maximum m and sum, and join at the end.
+// first splits, the only ones of short sequences, spread over all XCDs (16 sequences of 128 to 32,768 slots: 150 us
+// with splits first, 119 so).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its
+// own running maximum m and sum, and join at the end.
 //   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16,
 //     k = l / 16) holds dims 64 c + 16 k .. + 15 of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
 //   - O^T = V^T . P^T: those probabilities are the B operand where they lie, if the 32 slots of an MFMA
@@ -455,8 +468,12 @@ constexpr float kPScale = 16384.0f;    // probabilities enter the value product 
 //     those slots, which it reads as one piece of a row, and turns round by byte permutations while they
 //     become halves.  Row i's dims (D / 4) k .. are its outputs.
 //   - Codes are exact in fp16; a key block's scale multiplies its scores, a value block's the probabilities, under
-//     the largest value scale so far (vref) and kPScale, so that they neither overflow nor lose bits.
+//     the largest value scale of the split (vref) and kPScale, so that they neither overflow nor lose bits.
 //   - With several splits each writes m, the sum and its unnormalised rows; k_attend_join puts them together.
+// Bound by memory: those 16 sequences (8 kv heads of 128, 2 rows each, 540 MB) at 4.5 TB/s; 131,001 slots of 4 kv heads of
+// 64 (67 MB) 17 us; 2,049 slots of 8 kv heads 7.8, where it is the chain of a length, a tile and the waves' join.  The next
+// tile's keys go out when this one's scores are formed, its values when this one's product is: two whole tiles
+// in registers leave one wave a SIMD and take 135 us where this takes 119; 3 waves a SIMD spill (300).
 template <int D, int RT>
 __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
@@ -509,7 +526,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         fetch_v(first);
     }
     h8v q[RT][NC];
-    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
+    float qs[RT], m[RT], sum[RT];
     int lim[RT];
     f4 o[RT][NJ];
 #pragma unroll
@@ -525,6 +542,8 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
+    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
+    const float vscale = vref > 0.0f ? kPScale / vref : 0.0f;
     const int lim_all = row_limit(a, len, n, 0);    // slots that every row sees
     for (int tile = first; tile < t1; tile += 4) {
         f4 sc[RT][4];
@@ -547,13 +566,6 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
             vs[b] = __int_as_float(__builtin_amdgcn_readlane(sl, 4 + b));
         }
         if (tile + 4 < t1) fetch_k(tile + 4);
-        const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-        float vmove = 1.0f;
-        if (vtop > vref) {
-            vmove = vref / vtop;
-            vref = vtop;
-            vscale = kPScale / vref;
-        }
         h8v p[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -579,9 +591,6 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) o[r][j] *= move;
             }
-            if (vmove != 1.0f)
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) o[r][j] *= vmove;
             const float base = m[r] == -INFINITY ? 0.0f : m[r];
             float add[4];
             uint32_t pw[4][2];
@@ -714,6 +723,8 @@ __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
 // The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores were
 // kept; kv heads; sequences): D / 4 lanes a split, many
 // splits of one row (MANY) by 1024 / D groups whose sums are added in order, or a row a group.
+// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 4 splits 12 us, 2 rows of 128 (sequence,
+// head)s and their weights (34 MB of scores and sums) 12.5, 8 rows in 256 splits 5.
 template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     constexpr int LN = D / 4, GR = 256 / LN;
@@ -784,6 +795,12 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 // Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to LDS
 // at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the MFMAs of
 // these: left to itself the compiler waits for each read alone.
+// Bound by the vector ALU: a wave and tile of 64 MFMAs (1,000 clocks) has 490 vector instructions (2,300 clocks: 32
+// exponentials, 5 more instructions a score, 100 to turn codes into halves), and two waves a SIMD overlap the two in part.
+// 2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 45 us and 12 for the join; 3 x 209 rows over 4,001 to
+// 12,011 slots (41 GFLOP) 104 us.  Measured and not kept: eight waves of 16 rows (115 us: operands are read twice as
+// often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a second
+// form), the next tile's scores beside this tile's exponentials (124: no registers left for operand reads), wave priorities (no change).
 template <int D>
 __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
     constexpr int RT = 2, NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
@@ -860,7 +877,7 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
         fetch_v(t0);
     }
     h8v q[RT][NC];
-    float qs[RT], m[RT], sum[RT], vref = 0.0f, vscale = 0.0f;
+    float qs[RT], m[RT], sum[RT];
     int lim[RT];
     f4 o[RT][NJ];
 #pragma unroll
@@ -876,6 +893,8 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
+    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
+    const float vscale = vref > 0.0f ? kPScale / vref : 0.0f;
     auto step = [&](int tile, auto masked) {
         const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
         fetch_k(tile + 1);
@@ -905,14 +924,7 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 #pragma unroll
                     for (int r = 0; r < RT; ++r) sc[r][b] = mfma32(kf[c & 1][b], q[r][c], c ? sc[r][b] : (f4){0.f, 0.f, 0.f, 0.f});
             }
-            const float vtop = fmaxf(fmaxf(vs[0], vs[1]), fmaxf(vs[2], vs[3]));
-            float vmove = 1.0f;
-            if (vtop > vref) {
-                vmove = vref / vtop;
-                vref = vtop;
-                vscale = kPScale / vref;
-            }
-            bool grows = vmove != 1.0f;
+            bool grows = false;
             float top[RT];
 #pragma unroll
             for (int r = 0; r < RT; ++r) {
@@ -937,7 +949,7 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
                     m[r] = mn;
                     sum[r] *= move;
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) o[r][j] *= move * vmove;
+                    for (int j = 0; j < NJ; ++j) o[r][j] *= move;
                 }
             }
             // chunk 4u + k of dim 16 j + i: at (4 (u ^ j % 2) + k) ^ (i / 4) ^ 2 (i % 4)
@@ -1024,8 +1036,10 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 // acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels
 // left.  Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that none
 // is above its row's maximum; K in registers, the next 16 rows on their way while these are worked on; the sum over rows
-// is one over lanes i, in order of the row tiles.  Bound by the vector ALU (an exponential a score) and, at 3 waves a
-// SIMD, by its last turn; 128 slots a wave would need half the row reads, but one wave a SIMD: 100 us where this takes 55.
+// is one over lanes i, in order of the row tiles.  A second pass over K rather than kept scores, which from 9 rows on are
+// as many bytes as the keys and values.  Bound by the vector ALU (an exponential a score) and, at 3 waves a
+// SIMD, by its last turn: 3 x 209 rows over 4,001 to 12,011 slots 54 us; 128 slots a wave need half the row reads,
+// but leave one wave a SIMD: 100.
 // grid (slot tiles / 4 * by, kv heads, sequences): `by` (1, 2 or 4) waves take the row tiles of one slot tile in turn and
 // add up in their order.
 template <int D>
@@ -1140,7 +1154,8 @@ struct EvictLds {
 // between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in slot
 // order, of those at the threshold the first ones: counts of 64 slots each by ballots, one prefix sum over them, and the
 // place of each slot by the lanes before it.  R slots a thread at a time (slot base + 1,024 r + thread): if they are all
-// there are, weights are read once.
+// there are, weights are read once.  4 for up to 4,096 slots (2,049 slots: 9 us), else 32 (16 x 8 heads of 9,000 to 32,768
+// slots: 50 us, bound by one workgroup's chain of four counts; 95 with weights read each time and numbered 1,024 at a time).
 template <int R>
 __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, const float * acc, int len, int32_t * kept) {
     constexpr int kAt = R * kEvT;
@@ -1275,7 +1290,9 @@ __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
 constexpr int kMove = 64;                           // kept slots a workgroup of k_evict_move
 
 // grid (kept slots / 64, kv heads, sequences).  One wave looks up the slots' old places and scales, and the new scales
-// (the largest of each 16); then the codes, 16 bytes a thread at a time, all of a thread's on their way at once.
+// (the largest of each 16); then the codes, 16 bytes a thread at a time, all of a thread's on their way at once.  Bound by
+// memory: 16 x 8 heads of 12,001 slots (790 MB) 158 us, 5.0 TB/s; a workgroup a block of 16, each thread looking up its
+// own scales, took 431.
 template <int D>
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
     constexpr int CH = D / 16, N = 2 * kMove * CH / 256;    // 16-byte pieces of a row; pieces a thread
@@ -1331,7 +1348,8 @@ struct ReadArgs {
     void * k, * v;
 };
 
-// grid (values / 8 / 256 of one sequence and of K or V, K or V, sequences): 8 values a thread.
+// grid (values / 8 / 256 of one sequence and of K or V, K or V, sequences): 8 values a thread.  Bound by memory: 1.18 GB
+// (the 16 x 8 heads above, to fp16) 225 us, 5.2 TB/s.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_read(ReadArgs a) {
     const int is_v = blockIdx.y, s = blockIdx.z, H = a.c.n_kv_head;
