@@ -1599,7 +1599,11 @@ int q3t_dev_kv_reserve(q3t_dev * c, int32_t n_ctx) {
             return -1;
         HIP_OK(hipMemsetAsync(c->kv8, 0, g.n_layers * c->kv8_layer, c->stream));
         HIP_OK(hipMemsetAsync(c->kv8_at, 0, 4 * sizeof(int32_t), c->stream));
-        if (kv8_freqs(c) || ensure_kv8(c, 4)) return -1;
+        if (kv8_freqs(c) || ensure_kv8(c, 4)) {
+            dev_free(c, c->kv8);
+            c->kv8 = nullptr;
+            return -1;
+        }
     } else {
         if (dev_alloc_t(c, &c->kc, kv) || dev_alloc_t(c, &c->vc, kv) || dev_alloc_t(c, &c->probs, (size_t) g.n_head * n_ctx))
             return -1;
@@ -1715,6 +1719,7 @@ int q3t_dev_kv_write(q3t_dev * c, int32_t layer, int32_t n_pos, const uint16_t *
     if (layer < 0 || layer >= g.n_layers || n_pos < 0 || n_pos > c->n_ctx) return fail(c, "kv_write out of range");
     HIP_OK(hipSetDevice(c->device));
     if (c->kv_i8) {
+        if (!n_pos) return 0;
         if (check_room(c, 0, n_pos)) return -1;
         const size_t row = (size_t) g.n_kv_head * g.head_dim, bytes = n_pos * row * 2;
         uint16_t * d = nullptr;
@@ -3767,6 +3772,8 @@ int q3t_dev_stream_prefill(q3t_dev * c, int32_t stream, const float * embd, int3
 int q3t_dev_streams_begin(q3t_dev * c, const q3t_frame_args * args) {
     if (!c || !args) return -1;
     if (c->nb < 1) return fail(c, "q3t_dev_streams_reserve first");
+    // an 8-bit cache's rotary table ends behind the code predictor's positions
+    if (c->kv_i8) return fail(c, "multi-stream decode keeps an F16 talker cache (q3t_dev_kv_set_type F16 first)");
     if (c->n_ctx != c->sb_ctx) return fail(c, "KV cache re-reserved since q3t_dev_streams_reserve; reserve the streams again");
     HIP_OK(hipSetDevice(c->device));
     // the table keeps its address when rebuilt, so a captured frame graph stays valid

@@ -257,6 +257,43 @@ def test_restart_and_switches():
     ref.close()
 
 
+def test_streams_reserved_before_the_type_changed():
+    """Streams hold F16 caches: not begun, written or prefilled while the type is I8, and as before after it."""
+    cfg = qcfg.tiny()
+    dev = device("q8_0", F16, 64)
+    x = rows(cfg, 12, 3)
+    dev.streams_reserve(2, 64)
+    codes = []
+    for kind in (F16, I8, F16):
+        dev.kv_set_type(kind)
+        args = [dict(trailing=x[:2], tts_pad=x[4], n_past=10, max_len=6), dict(trailing=x[:3], tts_pad=x[5], n_past=12, max_len=6)]
+        if kind == I8:
+            for call in (lambda: dev.stream_prefill(0, x), lambda: dev.streams_begin(args)):
+                with pytest.raises(DeviceError, match="multi-stream"):
+                    call()
+            continue
+        dev.stream_prefill(0, x[:10])
+        dev.stream_prefill(1, x)
+        dev.streams_begin(args)
+        codes.append(dev.streams_run(6))
+    for a, b in zip(*(c[0] for c in codes)):
+        assert np.array_equal(a, b)
+    dev.close()
+
+
+def test_writing_no_rows_changes_nothing():
+    cfg = qcfg.tiny()
+    dev = device("q8_0", I8, 64)
+    dev.prefill(rows(cfg, 50, 1), 0)
+    dev.kv_evict(50, 20, 2, 4)
+    none = np.zeros((0, cfg.n_kv_head, cfg.head_dim), np.float16)
+    dev.kv_write(0, none, none)
+    with pytest.raises(DeviceError, match="eviction"):
+        dev.talker_step(rows(cfg, 1, 2)[0], 30)
+    dev.talker_step(rows(cfg, 1, 2)[0], 50)
+    dev.close()
+
+
 def test_refusals():
     cfg = qcfg.tiny()
     dev = device("q8_0", I8, 64)
