@@ -59,7 +59,9 @@ int check_cache(const q3t_kv8 * c, bool acc) {
     if (c->head_dim != 64 && c->head_dim != 128) return refuse("head_dim must be 64 or 128");
     if (c->n_seq < 1 || c->n_seq > 65535) return refuse("n_seq must be 1 to 65535");
     if (c->n_kv_head < 1 || c->n_kv_head > 4096) return refuse("n_kv_head must be 1 to 4096");
-    if (c->n_slots < 16 || c->n_slots % 16) return refuse("n_slots must be a positive multiple of 16");
+    // a grid's threads along one axis are counted in 32 bits: here, and in the bounds on rows and tokens below
+    if ((int64_t) c->n_seq * c->n_kv_head > 1 << 23) return refuse("n_seq * n_kv_head must be at most 2^23");
+    if (c->n_slots < 16 || c->n_slots % 16 || c->n_slots > 1 << 29) return refuse("n_slots must be a multiple of 16, 16 to 2^29");
     if (!is16(c->k) || !is16(c->v) || c->seq % 16 || c->head % 16) return refuse("codes must be 16-byte aligned");
     return 0;
 }
@@ -100,7 +102,7 @@ int q3t_kv8_rope(int32_t device, const q3t_kv8_rope_rows * rows, int32_t n, int6
     t_err[0] = 0;
     if (!rows || !freq) return refuse("null argument");
     if (n < 1 || n > 4) return refuse("1 to 4 tensors a call");
-    if (n_tokens < 0 || n_tokens > INT32_MAX) return refuse("n_tokens out of range");
+    if (n_tokens < 0 || n_tokens > 1 << 26) return refuse("n_tokens must be 0 to 2^26");
     if (head_dim < 16 || head_dim % 16 || head_dim > 256) return refuse("head_dim must be a multiple of 16, up to 256");
     if (rot_dim < 2 || rot_dim % 2 || rot_dim > head_dim) return refuse("rot_dim must be even, 2 to head_dim");
     kv8::RopeArgs a{};
@@ -131,7 +133,7 @@ int q3t_kv8_append(int32_t device, const q3t_kv8 * c, const void * k, const void
                    const int32_t * n_new, void * stream) {
     t_err[0] = 0;
     if (check_cache(c, false)) return -1;
-    if (n_rows < 0) return refuse("n_rows must not be negative");
+    if (n_rows < 0 || n_rows > 1 << 26) return refuse("n_rows must be 0 to 2^26");
     if (!n_rows) return 0;
     if (!k || !v) return refuse("null rows");
     if (!type_ok(type)) return refuse("type must be F32, F16 or BF16");
@@ -313,7 +315,8 @@ int q3t_kv8_read(int32_t device, const q3t_kv8 * c, const int32_t * start, int32
                  void * k, void * v, void * stream) {
     t_err[0] = 0;
     if (check_cache(c, false)) return -1;
-    if (n_rows < 0) return refuse("n_rows must not be negative");
+    if (n_rows < 0 || (int64_t) n_rows * c->n_kv_head * c->head_dim >= (int64_t) 1 << 35)
+        return refuse("n_rows must not be negative, nor n_rows * n_kv_head * head_dim 2^35");
     if (!type_ok(type)) return refuse("type must be F32, F16 or BF16");
     if (!is16(k) || !is16(v)) return refuse("outputs must be 16-byte aligned");
     if (!n_rows || (!k && !v)) return 0;
@@ -321,7 +324,6 @@ int q3t_kv8_read(int32_t device, const q3t_kv8 * c, const int32_t * start, int32
     kv8::ReadArgs a{*c, start, start0, n_rows, type, k, v};
     const int64_t per = (int64_t) n_rows * c->n_kv_head * c->head_dim;
     const int64_t blocks = (per / 8 + 255) / 256;
-    if (blocks > INT32_MAX) return refuse("too many rows");
     const dim3 grid((unsigned) blocks, 2, c->n_seq);
     auto go = [&](auto d, auto t) {
         hipLaunchKernelGGL((kv8::k_read<decltype(d)::value, decltype(t)::value>), grid, dim3(256), 0, (hipStream_t) stream, a);

@@ -189,7 +189,7 @@ __device__ __forceinline__ void rope_rows(const RopeArgs & a, const RopeRows & r
 // The angle pos * f in 64 bits, brought to [-pi, pi] by the nearest multiple of
 // 2 pi (as the sum of two doubles: |pos * f| < 2^31 turns leave 2^-50), and its
 // sine and cosine in fp32.
-__device__ __forceinline__ float2 rope_angle(int pos, double f, float mscale) {
+__device__ __forceinline__ float2 rope_angle(int64_t pos, double f, float mscale) {
     const double a = (double) pos * f;
     const double n = rint(a * 0.15915494309189535);
     double r = fma(-n, 6.283185307179586, a);
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(kRopeT) void k_rope(RopeArgs a) {
     const int nt = (int) min((int64_t) a.per, a.n_tokens - tok0), half = a.rot / 2;
     for (int i = threadIdx.x; i < nt * half; i += kRopeT) {
         const int64_t tok = tok0 + i / half;
-        const int pos = (a.pos ? a.pos[tok] : (int) tok) + a.pos0;
+        const int64_t pos = (a.pos ? a.pos[tok] : tok) + (int64_t) a.pos0;
         cs[i] = rope_angle(pos, a.freq[i % half], a.mscale);
     }
     __syncthreads();
@@ -270,7 +270,7 @@ __global__ __launch_bounds__(2 * D) void k_append(AppendArgs a) {
     const int64_t start = (int64_t) (a.start ? a.start[s] : 0) + a.start0;
     const int n = a.n_new ? min(max(a.n_new[s], 0), a.n_rows) : a.n_rows;
     const int64_t blk = (start >> 4) + blockIdx.x;
-    if (blk < 0 || blk >= a.c.n_slots / kBlk || blk * kBlk >= start + n) return;
+    if (!n || blk < 0 || blk >= a.c.n_slots / kBlk || blk * kBlk >= start + n) return;
     const int64_t i = blk * kBlk + r - start;          // the row of this thread's slot
     const bool fresh = i >= 0 && i < n;
     const bool begun = start > blk * kBlk;             // slots before start: only ever in the first block
@@ -448,9 +448,10 @@ __device__ __forceinline__ float max_rows(float x) {
 // A row's base of exponents follows its largest score only once that is more than this above it: a tile then needs
 // no exchange between lanes and no rescaling as a rule, and 2^1.9 kPScale is still an fp16 number.
 constexpr float kSlack = 1.9f;
-// The largest value scale of blocks b0 .. b1 - 1 (all 64 lanes).
+// The largest value scale of blocks b0 .. b1 - 1 (all 64 lanes), at least 2^-110: kPScale over it is then finite, and
+// smaller scales take the probabilities below kPScale, which costs bits from 2^-124 down.
 __device__ __forceinline__ float top_scale(const float * vs, int b0, int b1, int lane) {
-    float x = 0.0f;
+    float x = 0x1p-110f;
     for (int b = b0 + lane; b < b1; b += 64) x = fmaxf(x, vs[b]);
     return wave_max_f(x);
 }
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
     const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
-    const float vscale = vref > 0.0f ? kPScale / vref : 0.0f;
+    const float vscale = kPScale / vref;
     const int lim_all = row_limit(a, len, n, 0);    // slots that every row sees
     for (int tile = first; tile < t1; tile += 4) {
         f4 sc[RT][4];
@@ -714,7 +715,8 @@ __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
     for (int r = 0; r < 8; ++r)
         if (r < rows)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) add[e] = fmaf(__builtin_amdgcn_exp2f(x[r][e] - row_sum[r].x), row_sum[r].y, add[e]);
+            for (int e = 0; e < 4; ++e)             // a slot that the row does not see: unchanged, whatever the row's sum is
+                if (x[r][e] != -INFINITY) add[e] = fmaf(__builtin_amdgcn_exp2f(x[r][e] - row_sum[r].x), row_sum[r].y, add[e]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
         if (j + e < len) acc[e] = old[e] + add[e];
@@ -759,7 +761,8 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         __syncthreads();
         sum = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll 4
-        for (int x = gr; x < live; x += GR) o += *(const f4 *) (a.part + (cell + (int64_t) x * all_rows) * D + 4 * ln) * fac[x];
+        for (int x = gr; x < live; x += GR)
+            if (fac[x] != 0.0f) o += *(const f4 *) (a.part + (cell + (int64_t) x * all_rows) * D + 4 * ln) * fac[x];
         po[gr][ln] = o;
         __syncthreads();
         if (gr) return;
@@ -894,7 +897,7 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
     const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
-    const float vscale = vref > 0.0f ? kPScale / vref : 0.0f;
+    const float vscale = kPScale / vref;
     auto step = [&](int tile, auto masked) {
         const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
         fetch_k(tile + 1);
@@ -1100,7 +1103,7 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = __builtin_amdgcn_exp2f(sc[b][e] * (ks[b] * factor) - top);
-                        add[b][e] = fmaf(j0 + 16 * b + 4 * k + e < lim ? x : 0.0f, inv, add[b][e]);
+                        add[b][e] = j0 + 16 * b + 4 * k + e < lim ? fmaf(x, inv, add[b][e]) : add[b][e];
                     }
                 continue;
             }
@@ -1138,6 +1141,11 @@ struct EvictArgs {
 };
 
 constexpr int kEvT = 1024;
+
+__device__ __forceinline__ int evict_len(const EvictArgs & a, int s) {
+    const int64_t n = (int64_t) (a.lens ? a.lens[s] : 0) + a.len0;
+    return (int) min(max(n, (int64_t) 0), (int64_t) a.f.n_slots);
+}
 
 // An fp32 weight as an integer of the same order; -0 as +0, NaN as -infinity.
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -1273,10 +1281,8 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
 __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
     __shared__ EvictLds z;
     const int t = threadIdx.x, h = blockIdx.x, s = blockIdx.y;
-    const int64_t want_len = (int64_t) (a.lens ? a.lens[s] : 0) + a.len0;
-    const int len = (int) min(max(want_len, (int64_t) 0), (int64_t) a.f.n_slots), left = min(len, a.keep);
+    const int len = evict_len(a, s), left = min(len, a.keep);
     int32_t * kept = a.kept + ((int64_t) s * a.f.n_kv_head + h) * a.keep;
-    if (h == 0 && t == 0 && a.len_out) a.len_out[s] = left;
     for (int i = left + t; i < a.keep; i += kEvT) kept[i] = -1;
     if (len <= a.keep) {
         for (int i = t; i < left; i += kEvT) kept[i] = i;
@@ -1301,6 +1307,8 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
     const int t = threadIdx.x, h = blockIdx.y, s = blockIdx.z, at = blockIdx.x * kMove;
     const int32_t * kept = a.kept + ((int64_t) s * a.f.n_kv_head + h) * a.keep;
     const int64_t fsc = s * a.f.scale_seq + h * a.f.scale_head, tsc = s * a.t.scale_seq + h * a.t.scale_head;
+    // here, where every head's selection has read the old lengths: len_out may be lens
+    if (t == 0 && h == 0 && blockIdx.x == 0 && a.len_out) a.len_out[s] = min(evict_len(a, s), a.keep);
     if (t < kMove) {
         const int slot = at + t, f = slot < a.keep ? kept[slot] : -1;
         from[t] = f;

@@ -197,6 +197,7 @@ def append(cache, k, v, start, n_new=None):
     a sequence's rows are rows (the rest is padding)."""
     s, h, _, d = cache.shape
     index, shape, stride, t = cache.index, k.shape, k.stride(), _TYPES.get(k.dtype)
+    _need(start is not None, "start must be given")
     if len(shape) != 4 or shape[0] != s or shape[2] != h or shape[3] != d:
         raise Kv8Error(f"rows must be [{s}, n, {h}, {d}]")
     if shape != v.shape or k.dtype is not v.dtype or stride != v.stride() or k.get_device() != index or \
@@ -219,6 +220,7 @@ def attend(cache, q, lens, *, scale=None, n_new=None, causal=True, weights=False
         raise Kv8Error(f"q must be [{s}, n, heads, {d}] with dense dims, on the cache's GPU")
     if out is None:
         out = torch.empty_like(q, dtype=dtype, memory_format=torch.contiguous_format)
+    _need(lens is not None, "lens must be given")
     ostride = out.stride()
     if out.shape != shape or out.get_device() != index or (ostride[3] != 1 and shape[1]):
         raise Kv8Error("out must have q's shape, with dense dims, on its GPU")
@@ -243,6 +245,7 @@ def evict(cache, to, lens, *, n_keep, n_sink=0, n_recent=0):
     index = cache.index
     _need(to.index == index, "both caches must be on one GPU")
     _need(n_keep >= 1, "n_keep must be at least 1")
+    _need(lens is not None, "lens must be given")
     kept = torch.empty(s, h, n_keep, dtype=torch.int32, device=cache.device)
     left = torch.empty(s, dtype=torch.int32, device=cache.device)
     _check((_lib or load_kv8_library()).q3t_kv8_evict(index, cache.ref, to.ref, _ints(lens, s, index, "lens"), 0, n_keep, n_sink,
@@ -251,7 +254,8 @@ def evict(cache, to, lens, *, n_keep, n_sink=0, n_recent=0):
 
 
 def read(cache, start, n, *, dtype=torch.float32):
-    """Values of slots start[s] .. + n of every head: (k, v), each [S, n, H, D] in `dtype`; 0 outside the cache."""
+    """Values of slots start[s] .. + n (start None: 0 ..) of every head: (k, v), each [S, n, H, D] in `dtype`; 0 outside
+    the cache."""
     s, h, _, d = cache.shape
     index = cache.index
     _need(dtype in _TYPES and n >= 0, "dtype must be float32, float16 or bfloat16, n not negative")

@@ -125,6 +125,18 @@ def test_rope_strides_and_in_place(inter):
     within(out, w, rope_bound(w, m, torch.float32))
 
 
+def test_rope_position_sums_past_32_bits():
+    """pos + pos0 beyond an int32."""
+    x = torch.randn(4, 2, 64, generator=gen(14), device="cuda")
+    pos, freq = ints([2 ** 31 - 1, 2 ** 31 - 50, 0, 7]), torch.from_numpy(kv8.rope_freqs(64, 1e6)).cuda()
+    y, pos0 = torch.empty_like(x), 2 ** 31 - 1
+    rows = kv8._pack_rope(x.data_ptr(), y.data_ptr(), 128, 64, 128, 64, 0, 2, 0, 0)
+    kv8._check(kv8.load_kv8_library().q3t_kv8_rope(x.get_device(), rows, 1, 4, 64, 64, 0, pos.data_ptr(), pos0, freq.data_ptr(),
+                                                   1.0, 0.0, kv8._stream(x.get_device())), "rope")
+    want, mag = rope64(x, pos.long() + pos0, freq, None, False, 1.0, 0.0)
+    within(y, want, rope_bound(want, mag, torch.float32))
+
+
 def test_rope_nothing_and_refusals():
     freq = torch.from_numpy(kv8.rope_freqs(64, 1e4)).cuda()
     y, = kv8.rope([torch.empty(0, 4, 64, device="cuda")], ints([]), freq)
@@ -242,6 +254,16 @@ def test_append_one_by_one_and_strided():
         within(got, x.double(), 8.1 * step.double()[..., None])
         # and as a rule far less: the scales of random rows grow a few times
         assert ((got - x).abs() / step[..., None]).mean() < 0.6
+
+
+def test_append_of_no_rows_writes_nothing():
+    """Sequences of padding alone, whatever their block's scale holds."""
+    c = kv8.empty(2, 1, 64, 64)
+    c.tensors[2].fill_(math.nan)
+    before = snapshot(c)
+    k = torch.randn(2, 3, 1, 64, device="cuda")
+    kv8.append(c, k, k, ints([5, 37]), n_new=ints([0, -2]))
+    assert all(torch.equal(a.view(torch.int8), b.view(torch.int8)) for a, b in zip(c.tensors, before))
 
 
 # ---------------------------------------------------------------- attention
@@ -457,12 +479,65 @@ def test_attend_offsets_past_32_bits():
     within(head, k.double(), (c.tensors[2][0, :, -3:].max() * 0.51).double())
 
 
+@pytest.mark.parametrize("n", [1, 6, 12, 40, 150])
+def test_attend_whatever_the_workspace_holds(n, monkeypatch):
+    """Ten splits of 8 tiles, the last begun among the rows' own slots, so that some rows see none of it; and one split."""
+    g = gen(n + 60)
+    c = fill(1, 1, 5008, 128, g, spread=0.3)
+    q = query(1, n, 1, 128, g, torch.float16, 2.0)
+
+    def of_nan(*size, dtype=None, device=None):
+        return torch.full(size, 0xff, dtype=dtype, device=device)
+
+    want = [check_attend(c, q, [m]) for m in (4608 + 20, 4608 + n, 300)]
+    monkeypatch.setattr(kv8.torch, "empty", of_nan)     # the workspace's
+    got = [check_attend(c, q, [m]) for m in (4608 + 20, 4608 + n, 300)]
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("size", [1e-33, 1e-36, 1e-38])
+def test_attend_tiny_values(n, size):
+    """Value scales down to fp32's subnormal numbers."""
+    g = gen(n + 70)
+    c = fill(2, 1, 400, 128, g)
+    c.tensors[3].mul_(size)
+    q = query(2, n, 2, 128, g, torch.float16, 2.0)
+    want, err, _, _ = attend64(c, q, [400, n + 7], None, True, 128 ** -0.5)
+    got = kv8.attend(c, q, ints([400, n + 7]), dtype=torch.float32)
+    # a probability times its scale is a multiple of 2^-24 at least of 2^-124: 127 * 2^-149 a slot; then the results'
+    # own rounding, to multiples of 2^-149 too, in up to four sums
+    within(got, want, err + want.abs() * U + (400 * 127 + 4) * 2.0 ** -149)
+
+
+@pytest.mark.parametrize("n", [5, 12, 60])
+def test_weights_of_rows_that_are_not_finite(n):
+    """Such a row makes the weights of the slots that it sees NaN, and no others."""
+    g = gen(n + 80)
+    c = fill(2, 2, 256, 64, g)
+    q = query(2, n, 4, 64, g, torch.float16)
+    q[:, 1] = 0.0
+    lens = [200, n]
+    before = c.tensors[4].clone()
+    kv8.attend(c, q, ints(lens), weights=True)
+    clean = c.tensors[4].clone()
+    q[0, 1, 0, 3] = math.nan            # of kv head 0
+    q[1, 1, 3, 60] = math.inf           # of kv head 1
+    c.tensors[4].copy_(before)
+    kv8.attend(c, q, ints(lens), weights=True)
+    seen = torch.zeros_like(clean, dtype=torch.bool)
+    seen[0, 0, :lens[0] - n + 2] = True
+    seen[1, 1, :2] = True
+    assert c.tensors[4][seen].isnan().all()
+    assert torch.equal(c.tensors[4][~seen], clean[~seen])
+
+
 def test_attend_refusals():
     c = fill(2, 2, 64, 64, gen(1), weights=False)
     q = torch.randn(2, 3, 4, 64, device="cuda").half()
     lens = ints([10, 20])
     for bad in [dict(q=q.float()), dict(q=q[:1]), dict(q=q[..., :32]), dict(q=q[:, :, :3]), dict(lens=ints([1])), dict(lens=lens.long()),
-                dict(lens=lens.cpu()), dict(weights=True), dict(max_len=65), dict(out=q[:, :2]), dict(out=q.double()),
+                dict(lens=lens.cpu()), dict(lens=None), dict(weights=True), dict(max_len=65), dict(out=q[:, :2]), dict(out=q.double()),
                 dict(n_new=ints([1])), dict(scale=math.nan), dict(q=q.transpose(2, 3).contiguous().transpose(2, 3))]:
         a = dict(q=q, lens=lens) | bad
         with pytest.raises(kv8.Kv8Error):
@@ -569,6 +644,19 @@ def test_evict_refuses_its_own_memory():
         kv8.evict(c, c, ints([64]), n_keep=10)
     with pytest.raises(kv8.Kv8Error, match="n_keep"):
         kv8.evict(c, fill(1, 1, 32, 64, gen(1)), ints([64]), n_keep=33)
+
+
+def test_evict_writes_the_lengths_in_place():
+    """len_out may be lens: every head reads the old length."""
+    g = gen(8)
+    c = fill(40, 8, 96, 64, g)
+    lens = [96 - s for s in range(40)]
+    to, kept, left = check_evict(c, lens, 33, 3, 5)
+    at, again, mine = ints(lens), torch.empty_like(kept), fill(40, 8, 48, 64, gen(99))
+    kv8._check(kv8.load_kv8_library().q3t_kv8_evict(c.index, c.ref, mine.ref, at.data_ptr(), 0, 33, 3, 5, again.data_ptr(),
+                                                    at.data_ptr(), kv8._stream(c.index)), "evict")
+    assert torch.equal(at, left) and torch.equal(again, kept)
+    assert all(torch.equal(a, b) for a, b in zip(to.tensors, mine.tensors))
 
 
 # ---------------------------------------------------------------- read

@@ -120,6 +120,17 @@ def test_append_evict_read_refuse():
     refused(lib.q3t_kv8_read(0, b(cache()), None, 0, 1, 0, P + 8, P, None), "aligned")
 
 
+def test_sizes_past_a_launch_are_refused():
+    lib, b = kv8.load_kv8_library(), ctypes.byref
+    refused(lib.q3t_kv8_attend_ws(b(cache(n_slots=(1 << 29) + 16)), b(attend_args())), "n_slots")
+    refused(lib.q3t_kv8_attend_ws(b(cache(n_seq=65535, n_kv_head=129)), b(attend_args())), "n_seq * n_kv_head")
+    assert lib.q3t_kv8_attend_ws(b(cache(n_slots=1 << 29)), b(attend_args(max_len=1 << 29))) > 0
+    refused(lib.q3t_kv8_append(0, b(cache()), P, P, 0, 0, 0, 0, (1 << 26) + 1, None, 0, None, None), "n_rows")
+    refused(lib.q3t_kv8_read(0, b(cache()), None, 0, 1 << 27, 0, P, P, None), "n_rows")
+    rows = (kv8.CRopeRows * 1)(kv8.CRopeRows(P, 2 * P, 256, 128, 256, 128, None, 2, 0, 1))
+    refused(rope_call(rows, tokens=(1 << 26) + 1), "n_tokens")
+
+
 def rope_call(rows, n=1, tokens=4, d=128, rot=128, freq=P):
     return kv8.load_kv8_library().q3t_kv8_rope(0, rows, n, tokens, d, rot, 0, None, 0, freq, 1.0, 1e-6, None)
 
