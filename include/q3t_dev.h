@@ -152,35 +152,35 @@ int32_t q3t_dev_kv_capacity(const q3t_dev * dev);
  * bfloat16 bits.
  *
  * Q3T_TYPE_I8 is the 8-bit cache of q3t_kv8.h: int8 codes with a scale for
- * each 16 slots of a head, 58,352 bytes a position instead of 114,688 for the 0.6B
- * talker, no bound on n_ctx but memory, and the attention weight every slot
- * draws kept with it, by which q3t_dev_kv_evict makes room.  Rows are
- * quantised as they are stored (q3t_dev_kv_write takes fp16 rows, and starts the
- * cache anew), q is
- * rounded to fp16, softmax and sums are fp32.  Positions are rotated by angles taken
- * in 64 bits, not from the table, so they may pass n_ctx.  Prefills,
- * single steps and the frame loop run on it, on the multi-kernel path; attention
- * capture and multi-stream decode refuse it. */
+ * each 16 slots of a head, 58,352 bytes a position instead of 114,688 for the
+ * 0.6B talker, no bound on n_ctx but memory, and the attention weight every
+ * slot draws kept with it, by which q3t_dev_kv_evict makes room.  Rows are
+ * quantised as they are stored (q3t_dev_kv_write takes fp16 rows, and starts
+ * the cache anew), q is rounded to fp16, softmax and sums are fp32.  Positions
+ * are rotated by angles taken in 64 bits, not from the table, so they may pass
+ * n_ctx.  Prefills, single steps and the frame loop run on it, on the
+ * multi-kernel path; attention capture and multi-stream decode refuse it. */
 int  q3t_dev_kv_set_type(q3t_dev * dev, int32_t type);
 /* I8 caches: keeps n_keep of the slots of each layer and KV head that the
- * n_past positions so far hold (all, if there are no more): the first n_sink, the
- * last n_recent and, of the rest, those that drew the most attention
- * weight; order and rotation stay.  The next position is n_past as before,
- * its slot n_keep.  Earlier positions cannot be written again, except that
- * position 0 starts the cache anew.  May be called between
- * q3t_dev_frames_run calls (n_past = the loop's n_past + the frames run): an I8
- * frame loop asks for room when it runs, not for max_len positions when it
- * begins.  kept_out (NULL ok): [n_layers][n_kv_head][n_keep] the kept slots' numbers
- * before, ascending, -1 behind them. */
+ * n_past positions so far hold (all, if there are no more): the first n_sink,
+ * the last n_recent and, of the rest, those that drew the most attention
+ * weight; order and rotation stay.  The next position is n_past as before, its
+ * slot n_keep.  Earlier positions cannot be written again, except that position
+ * 0 starts the cache anew.  May be called between q3t_dev_frames_run calls
+ * (n_past = the loop's n_past + the frames run): an I8 frame loop asks for room
+ * when it runs, not for max_len positions when it begins.  kept_out (NULL ok):
+ * [n_layers][n_kv_head][n_keep] the kept slots' numbers before, ascending, -1
+ * behind them. */
 int  q3t_dev_kv_evict(q3t_dev * dev, int32_t n_past, int32_t n_keep, int32_t n_sink, int32_t n_recent,
                       int32_t * kept_out);
 /* I8 caches: the values of slots [slot0, slot0 + n) of a talker layer, k and
- * v as [n][n_kv_head][head_dim], and the weight each has drawn, [n_kv_head][n] (any may be NULL). */
+ * v as [n][n_kv_head][head_dim], and the weight each has drawn,
+ * [n_kv_head][n] (any may be NULL). */
 int  q3t_dev_kv_read(q3t_dev * dev, int32_t layer, int32_t slot0, int32_t n, float * k, float * v, float * weight);
 /* I8 caches: rotary frequencies for contexts `factor` times the trained
- * n_trained positions (scaling as in q3t_kv8_rope_freqs, 0 = none; mscale multiplies
- * the rotated q and k, 1 = as trained).  Rows already stored keep their
- * rotation: call it before the first prefill. */
+ * n_trained positions (scaling as in q3t_kv8_rope_freqs, 0 = none; mscale
+ * multiplies the rotated q and k, 1 = as trained).  Rows already stored keep
+ * their rotation: call it before the first prefill. */
 int  q3t_dev_set_rope_scaling(q3t_dev * dev, int32_t scaling, double factor, int32_t n_trained, float mscale);
 /* Attention-row capture, the device side of set_attn_dump / attn_rows
  * (src/tts_transformer.h:224-227; rows captured in forward_step,

@@ -194,9 +194,9 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
         st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 16) + 3) & ~(int64_t) 3;
     } else {
         p.row_tiles = (int) ((rows + kv8::kTileRows - 1) / kv8::kTileRows);
-        // The shortest splits, of 8 tiles at least, with no more than 600 workgroups, were all sequences as long as the
-        // longest: two a CU run at once, and more would start a third turn.  2,049 rows and slots of 8 x 2 heads, splits
-        // of 8, 9, 10, 12, 17, 33 tiles: 68, 63, 58, 61, 66, 68 us with their joins.
+        // The shortest splits, of 8 tiles at least, with no more than 600 workgroups, were all sequences as long as
+        // the longest: two a CU run at once, and more would start a third turn.  2,049 rows and slots of 8 x 2 heads,
+        // splits of 8, 9, 10, 12, 17, 33 tiles: 68, 63, 58, 61, 66, 68 us with their joins.
         const int64_t before = a->causal ? std::max<int64_t>(len - a->n_rows, 0) : len;   // slots that row 0 does not add to
         auto groups = [&](int64_t of) {
             int64_t g = 0;
@@ -240,8 +240,8 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
     if (join.x && many) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), join, dim3(256), 0, st, a);
     else if (join.x) hipLaunchKernelGGL((kv8::k_attend_join<D, false>), join, dim3(256), 0, st, a);
     if (p.drawn) {
-        // waves that share a slot tile, where one a tile would leave CUs without work (each loads the tile's keys: 3 x 209
-        // rows over 12,011 slots, 1, 2, 4 waves: 55, 64, 80 us)
+        // waves that share a slot tile, where one a tile would leave CUs without work (each loads the tile's keys: 3
+        // x 209 rows over 12,011 slots, 1, 2, 4 waves: 55, 64, 80 us)
         const int64_t tiles = (a.max_len + 63) / 64, groups = tiles * H * S / 4;
         const int by = rows <= 48 || groups >= 512 ? 1 : groups >= 256 ? 2 : 4;
         hipLaunchKernelGGL(kv8::k_attend_drawn<D>, dim3((unsigned) ((tiles * by + 3) / 4), H, S), dim3(256), 0, st, a, by,

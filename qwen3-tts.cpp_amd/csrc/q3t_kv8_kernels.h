@@ -199,10 +199,11 @@ __device__ __forceinline__ float2 rope_angle(int64_t pos, double f, float mscale
     return make_float2(c * mscale, s * mscale);
 }
 
-// Bound by memory: 11,301 tokens of 36 heads (208 MB) 39 us, 2,049 tokens of 24 heads from fp32 to fp16 (38 MB) 10 us,
-// one token 4.8 us.  All rows through LDS took 106, 20 and 5.6: words 16 apart in the banks, and the angles once a tensor.
-// grid (tokens / per).  A workgroup takes `per` tokens: their sines and cosines once for all heads of all tensors, then
-// the rows.
+// Bound by memory: 11,301 tokens of 36 heads (208 MB) 39 us, 2,049 tokens of 24 heads from fp32 to fp16 (38 MB) 10
+// us, one token 4.8 us.  All rows through LDS took 106, 20 and 5.6: words 16 apart in the banks, and the angles once
+// a tensor.
+// grid (tokens / per).  A workgroup takes `per` tokens: their sines and cosines once for all heads of all tensors,
+// then the rows.
 __global__ __launch_bounds__(kRopeT) void k_rope(RopeArgs a) {
     __shared__ float2 cs[kRopeTok * kRopeMax];
     __shared__ float rows[kRopeT * 17];
@@ -317,7 +318,8 @@ struct AttendArgs {
     int32_t row_blocks;                 // k_attend_join: workgroups of a sequence and kv head that take rows
     int32_t score_len, rows16;          // scores a row; rows to a multiple of 16
     // workspace, each where the call needs it: [seq][kv head][split][row][D]; [..][row]: maximum, sum; [seq][kv
-    // head][row][score_len]; [seq][kv head][rows16][D]: q in fp16; [seq][kv head][rows16]: its factor, the row's maximum, 1 / its sum
+    // head][row][score_len]; [seq][kv head][rows16][D]: q in fp16; [seq][kv head][rows16]: its factor, the row's
+    // maximum, 1 / its sum
     float * part; float2 * stat; float * score; uint16_t * qh; f4 * rowq;
 };
 
@@ -361,9 +363,10 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// One row of q as MFMA operands: this lane's dims off + lo (c % 2) + hi (c / 2) .. + 7 in q[c], in fp16 under the power of two that
-// brings the row's largest value to [1, 2) (exact for fp16, and for all bits of bfloat16 values down to 2^-14 of the
-// largest), with the sign of the scale.  Returns the factor of a product with it (not negative), NaN for a row that is not finite.
+// One row of q as MFMA operands: this lane's dims off + lo (c % 2) + hi (c / 2) .. + 7 in q[c], in fp16 under the
+// power of two that brings the row's largest value to [1, 2) (exact for fp16, and for all bits of bfloat16 values
+// down to 2^-14 of the largest), with the sign of the scale.  Returns the factor of a product with it (not negative),
+// NaN for a row that is not finite.
 template <int D>
 __device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, int off, int lo, int hi,
                                              h8v (&q)[D / 32]) {
@@ -460,21 +463,21 @@ constexpr float kPScale = 16384.0f;    // probabilities enter the value product 
 // Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), four
 // waves; workgroups go to the XCDs in turn, so heads come first and a sequence's splits are turned by its number: the
 // first splits, the only ones of short sequences, spread over all XCDs (16 sequences of 128 to 32,768 slots: 150 us
-// with splits first, 119 so).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with its
-// own running maximum m and sum, and join at the end.
-//   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16,
-//     k = l / 16) holds dims 64 c + 16 k .. + 15 of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
-//   - O^T = V^T . P^T: those probabilities are the B operand where they lie, if the 32 slots of an MFMA
-//     are taken as 4k + e of one block of 16, then of the next; lane (i, k) then needs the codes of dims (D / 16) i .. of
-//     those slots, which it reads as one piece of a row, and turns round by byte permutations while they
-//     become halves.  Row i's dims (D / 4) k .. are its outputs.
+// with splits first, 119 so).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with
+// its own running maximum m and sum, and join at the end.
+//   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16, k
+//     = l / 16) holds dims 64 c + 16 k .. + 15 of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
+//   - O^T = V^T . P^T: those probabilities are the B operand where they lie, if the 32 slots of an MFMA are taken as
+//     4k + e of one block of 16, then of the next; lane (i, k) then needs the codes of dims (D / 16) i .. of those
+//     slots, which it reads as one piece of a row, and turns round by byte permutations while they become halves.
+//     Row i's dims (D / 4) k .. are its outputs.
 //   - Codes are exact in fp16; a key block's scale multiplies its scores, a value block's the probabilities, under
 //     the largest value scale of the split (vref) and kPScale, so that they neither overflow nor lose bits.
 //   - With several splits each writes m, the sum and its unnormalised rows; k_attend_join puts them together.
-// Bound by memory: those 16 sequences (8 kv heads of 128, 2 rows each, 540 MB) at 4.5 TB/s; 131,001 slots of 4 kv heads of
-// 64 (67 MB) 17 us; 2,049 slots of 8 kv heads 7.8, where it is the chain of a length, a tile and the waves' join.  The next
-// tile's keys go out when this one's scores are formed, its values when this one's product is: two whole tiles
-// in registers leave one wave a SIMD and take 135 us where this takes 119; 3 waves a SIMD spill (300).
+// Bound by memory: those 16 sequences (8 kv heads of 128, 2 rows each, 540 MB) at 4.5 TB/s; 131,001 slots of 4 kv
+// heads of 64 (67 MB) 17 us; 2,049 slots of 8 kv heads 7.8, where it is the chain of a length, a tile and the waves'
+// join.  The next tile's keys go out when this one's scores are formed, its values when this one's product is: two
+// whole tiles in registers leave one wave a SIMD and take 135 us where this takes 119; 3 waves a SIMD spill (300).
 template <int D, int RT>
 __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
@@ -722,11 +725,11 @@ __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
         if (j + e < len) acc[e] = old[e] + add[e];
 }
 
-// The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores were
-// kept; kv heads; sequences): D / 4 lanes a split, many
-// splits of one row (MANY) by 1024 / D groups whose sums are added in order, or a row a group.
-// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 4 splits 12 us, 2 rows of 128 (sequence,
-// head)s and their weights (34 MB of scores and sums) 12.5, 8 rows in 256 splits 5.
+// The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores
+// were kept; kv heads; sequences): D / 4 lanes a split, many splits of one row (MANY) by 1024 / D groups whose sums
+// are added in order, or a row a group.
+// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 4 splits 12 us, 2 rows of 128
+// (sequence, head)s and their weights (34 MB of scores and sums) 12.5, 8 rows in 256 splits 5.
 template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     constexpr int LN = D / 4, GR = 256 / LN;
@@ -788,22 +791,23 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 
 // ----------------------------------------------- attention of many rows
 // A tile of 128 rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
-// fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four waves of
-// 32 rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
+// fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four
+// waves of 32 rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
 // k_attend_few; here all waves go through the same tiles, with dims in their own order:
 //   K in LDS: [slot][dim] in 16-byte chunks, chunk c of slot t at c ^ (t % (D / 8));
-//   V in LDS: [dim][8 chunks], chunk 4u + k = slots 32u + 4k + e, then 32u + 16 + 4k + e (an operand of the
-//   value product as it is), at chunk ^ f(dim) with f = (dim / 4) % 8 ^ 2 (dim % 4), so that both the 16 dims of a
-//   read and the 32 dim quads of a write spread over all banks.
-// Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to LDS
-// at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the MFMAs of
-// these: left to itself the compiler waits for each read alone.
+//   V in LDS: [dim][8 chunks], chunk 4u + k = slots 32u + 4k + e, then 32u + 16 + 4k + e (an operand of the value
+//   product as it is), at chunk ^ f(dim) with f = (dim / 4) % 8 ^ 2 (dim % 4), so that both the 16 dims of a read and
+//   the 32 dim quads of a write spread over all banks.
+// Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to
+// LDS at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the
+// MFMAs of these: left to itself the compiler waits for each read alone.
 // Bound by the vector ALU: a wave and tile of 64 MFMAs (1,000 clocks) has 490 vector instructions (2,300 clocks: 32
-// exponentials, 5 more instructions a score, 100 to turn codes into halves), and two waves a SIMD overlap the two in part.
-// 2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 45 us and 12 for the join; 3 x 209 rows over 4,001 to
-// 12,011 slots (41 GFLOP) 104 us.  Measured and not kept: eight waves of 16 rows (115 us: operands are read twice as
-// often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a second
-// form), the next tile's scores beside this tile's exponentials (124: no registers left for operand reads), wave priorities (no change).
+// exponentials, 5 more instructions a score, 100 to turn codes into halves), and two waves a SIMD overlap the two in
+// part. 2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 45 us and 12 for the join; 3 x 209 rows over
+// 4,001 to 12,011 slots (41 GFLOP) 104 us.  Measured and not kept: eight waves of 16 rows (115 us: operands are read
+// twice as often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a
+// second form), the next tile's scores beside this tile's exponentials (124: no registers left for operand reads),
+// wave priorities (no change).
 template <int D>
 __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
     constexpr int RT = 2, NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
@@ -1037,14 +1041,14 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 }
 
 // acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels
-// left.  Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that none
-// is above its row's maximum; K in registers, the next 16 rows on their way while these are worked on; the sum over rows
-// is one over lanes i, in order of the row tiles.  A second pass over K rather than kept scores, which from 9 rows on are
-// as many bytes as the keys and values.  Bound by the vector ALU (an exponential a score) and, at 3 waves a
-// SIMD, by its last turn: 3 x 209 rows over 4,001 to 12,011 slots 54 us; 128 slots a wave need half the row reads,
-// but leave one wave a SIMD: 100.
-// grid (slot tiles / 4 * by, kv heads, sequences): `by` (1, 2 or 4) waves take the row tiles of one slot tile in turn and
-// add up in their order.
+// left.  Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that
+// none is above its row's maximum; K in registers, the next 16 rows on their way while these are worked on; the sum
+// over rows is one over lanes i, in order of the row tiles.  A second pass over K rather than kept scores, which from
+// 9 rows on are as many bytes as the keys and values.  Bound by the vector ALU (an exponential a score) and, at 3
+// waves a SIMD, by its last turn: 3 x 209 rows over 4,001 to 12,011 slots 54 us; 128 slots a wave need half the row
+// reads, but leave one wave a SIMD: 100.
+// grid (slot tiles / 4 * by, kv heads, sequences): `by` (1, 2 or 4) waves take the row tiles of one slot tile in turn
+// and add up in their order.
 template <int D>
 __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int lo) {
     constexpr int NC = D / 32, NB = 4;
@@ -1074,7 +1078,8 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
         }
         // the first row that sees slot j0
         const int rt0 = (a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0) + w % by, rt1 = (rows + 15) / 16;
-        // from this row on a row sees all of these slots: none is masked (a row past the last one has a finite row's scores)
+        // from this row on a row sees all of these slots: none is masked (a row past the last one has a finite row's
+        // scores)
         const int clear = a.causal ? max(j0 + 63 - (len - n), 0) * a.group : 0;
         const uint16_t * qb = a.qh + hd * a.rows16 * D;
         const f4 * rb = a.rowq + hd * a.rows16;
@@ -1159,11 +1164,12 @@ struct EvictLds {
 };
 
 // The kept slots of one head with more than `keep` of them.  The threshold (the want-th largest weight of the slots
-// between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in slot
-// order, of those at the threshold the first ones: counts of 64 slots each by ballots, one prefix sum over them, and the
-// place of each slot by the lanes before it.  R slots a thread at a time (slot base + 1,024 r + thread): if they are all
-// there are, weights are read once.  4 for up to 4,096 slots (2,049 slots: 9 us), else 32 (16 x 8 heads of 9,000 to 32,768
-// slots: 50 us, bound by one workgroup's chain of four counts; 95 with weights read each time and numbered 1,024 at a time).
+// between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in
+// slot order, of those at the threshold the first ones: counts of 64 slots each by ballots, one prefix sum over them,
+// and the place of each slot by the lanes before it.  R slots a thread at a time (slot base + 1,024 r + thread): if
+// they are all there are, weights are read once.  4 for up to 4,096 slots (2,049 slots: 9 us), else 32 (16 x 8 heads
+// of 9,000 to 32,768 slots: 50 us, bound by one workgroup's chain of four counts; 95 with weights read each time and
+// numbered 1,024 at a time).
 template <int R>
 __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, const float * acc, int len, int32_t * kept) {
     constexpr int kAt = R * kEvT;
@@ -1295,10 +1301,10 @@ __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
 
 constexpr int kMove = 64;                           // kept slots a workgroup of k_evict_move
 
-// grid (kept slots / 64, kv heads, sequences).  One wave looks up the slots' old places and scales, and the new scales
-// (the largest of each 16); then the codes, 16 bytes a thread at a time, all of a thread's on their way at once.  Bound by
-// memory: 16 x 8 heads of 12,001 slots (790 MB) 158 us, 5.0 TB/s; a workgroup a block of 16, each thread looking up its
-// own scales, took 431.
+// grid (kept slots / 64, kv heads, sequences).  One wave looks up the slots' old places and scales, and the new
+// scales (the largest of each 16); then the codes, 16 bytes a thread at a time, all of a thread's on their way at
+// once.  Bound by memory: 16 x 8 heads of 12,001 slots (790 MB) 158 us, 5.0 TB/s; a workgroup a block of 16, each
+// thread looking up its own scales, took 431.
 template <int D>
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
     constexpr int CH = D / 16, N = 2 * kMove * CH / 256;    // 16-byte pieces of a row; pieces a thread
@@ -1356,8 +1362,8 @@ struct ReadArgs {
     void * k, * v;
 };
 
-// grid (values / 8 / 256 of one sequence and of K or V, K or V, sequences): 8 values a thread.  Bound by memory: 1.18 GB
-// (the 16 x 8 heads above, to fp16) 225 us, 5.2 TB/s.
+// grid (values / 8 / 256 of one sequence and of K or V, K or V, sequences): 8 values a thread.  Bound by memory: 1.18
+// GB (the 16 x 8 heads above, to fp16) 225 us, 5.2 TB/s.
 template <int D, int T>
 __global__ __launch_bounds__(256) void k_read(ReadArgs a) {
     const int is_v = blockIdx.y, s = blockIdx.z, H = a.c.n_kv_head;
