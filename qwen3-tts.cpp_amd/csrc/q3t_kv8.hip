@@ -176,8 +176,8 @@ namespace {
 // How a call runs: its kernels, splits and the parts of its workspace (bytes).
 struct AttendPlan {
     bool few, scored, drawn;
-    int rt, row_tiles, split_tiles, n_split, score_len, rows16;
-    int64_t part, stat, score, qh, rowq, total;
+    int rt, row_tiles, units, split_tiles, n_split, score_len, rows16;
+    int64_t part, stat, split, score, qh, rowq, total;
 };
 
 AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
@@ -193,31 +193,25 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
         // 4 tiles (one a wave) to 16 a split, so that there are about 1,024 workgroups: four a CU
         st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 16) + 3) & ~(int64_t) 3;
     } else {
+        // As many workgroups as run at once, two a CU, or splits of 8 tiles if those are fewer: more start a second turn
+        // (512, 640, 768, 1,024: 3 x 209 rows over 4,001 to 12,011 slots 84, 92, 85, 91 us, 2,049 rows over their own
+        // 49, 56, 57, 57).
         p.row_tiles = (int) ((rows + kv8::kTileRows - 1) / kv8::kTileRows);
-        // The shortest splits, of 8 tiles at least, with no more than 600 workgroups, were all sequences as long as
-        // the longest: two a CU run at once, and more would start a third turn.  2,049 rows and slots of 8 x 2 heads,
-        // splits of 8, 9, 10, 12, 17, 33 tiles: 68, 63, 58, 61, 66, 68 us with their joins.
-        const int64_t before = a->causal ? std::max<int64_t>(len - a->n_rows, 0) : len;   // slots that row 0 does not add to
-        auto groups = [&](int64_t of) {
-            int64_t g = 0;
-            for (int64_t r = 0; r < p.row_tiles; ++r) {
-                const int64_t slots = std::min(len, before + (std::min((r + 1) * kv8::kTileRows, rows) + group - 1) / group);
-                g += ((slots + 63) / 64 + of - 1) / of;
-            }
-            return g * heads;
-        };
-        st = 8;
-        while (st < tiles && groups(st) > 600) st += std::max<int64_t>(st / 8, 1);
-        st = std::min(st, std::max<int64_t>(tiles, 1));
+        const int64_t whole = heads * p.row_tiles;
+        p.units = whole < kv8::kUnits ? (int) std::min<int64_t>(kv8::kUnits, whole * ((tiles + 7) / 8)) : 0;
+        if (p.units == whole) p.units = 0;
+        st = tiles;
     }
-    st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
+    if (p.few) st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
     p.split_tiles = (int) st;
     p.n_split = (int) ((tiles + st - 1) / st);
     p.score_len = (int) std::min<int64_t>(tiles * 64, INT32_MAX);
     p.rows16 = (int) ((rows + 15) / 16 * 16);
     auto take = [&](int64_t bytes) { const int64_t at = p.total; p.total += (bytes + 255) / 256 * 256; return at; };
-    if (p.n_split > 1) p.part = take(heads * p.n_split * rows * c->head_dim * 4);
-    if (p.n_split > 1 || p.scored) p.stat = take(heads * p.n_split * rows * 8);
+    const int64_t cells = p.units ? (int64_t) p.units * kv8::kTileRows : heads * p.n_split * rows;
+    if (p.units || p.n_split > 1) p.part = take(cells * c->head_dim * 4);
+    if (p.units || p.n_split > 1 || p.scored) p.stat = take(cells * 8);
+    if (p.units) p.split = take(heads * p.row_tiles * 8);
     if (p.scored) p.score = take(heads * rows * p.score_len * 4);
     if (p.drawn) p.qh = take(heads * p.rows16 * c->head_dim * 2);
     if (p.drawn) p.rowq = take(heads * p.rows16 * 16);
@@ -232,10 +226,10 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
         if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1>), grid, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((kv8::k_attend_few<D, 2>), grid, dim3(256), 0, st, a);
     } else {
-        hipLaunchKernelGGL(kv8::k_attend_tile<D>, dim3(H * S, p.row_tiles, p.n_split), dim3(kv8::kTileT), 0, st, a);
+        hipLaunchKernelGGL(kv8::k_attend_tile<D>, p.units ? dim3(p.units) : dim3(H * S, p.row_tiles), dim3(kv8::kTileT), 0, st, a);
     }
-    const bool many = p.n_split > 8;
-    a.row_blocks = p.n_split == 1 ? 0 : many ? rows : (rows + 1024 / D - 1) / (1024 / D);
+    const bool many = p.few ? p.n_split > 8 : p.units > 8 * H * S * p.row_tiles;
+    a.row_blocks = p.n_split == 1 && !p.units ? 0 : many ? rows : (rows + 1024 / D - 1) / (1024 / D);
     const dim3 join(a.row_blocks + (p.scored ? (a.max_len + 1023) / 1024 : 0), H, S);
     if (join.x && many) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), join, dim3(256), 0, st, a);
     else if (join.x) hipLaunchKernelGGL((kv8::k_attend_join<D, false>), join, dim3(256), 0, st, a);
@@ -275,14 +269,18 @@ int q3t_kv8_attend(int32_t device, const q3t_kv8 * c, const q3t_kv8_attend_args 
     a.lens = p->lens; a.n_new = p->n_new; a.len0 = p->len0; a.q_type = p->q_type; a.o_type = p->o_type;
     a.n_rows = p->n_rows; a.n_head = p->n_head; a.group = p->n_head / c->n_kv_head;
     a.max_len = p->max_len ? p->max_len : c->n_slots;
+    a.per_group = 1.0f / a.group;
     a.causal = p->causal != 0; a.weights = p->weights != 0; a.scale = p->scale;
     a.qvec = is16(p->q) && strides16(p->q_type, {p->q_seq, p->q_row, p->q_head});
     a.ovec = is16(p->out) && strides16(p->o_type, {p->o_seq, p->o_row, p->o_head});
     a.split_tiles = plan.split_tiles; a.n_split = plan.n_split; a.row_tiles = plan.row_tiles;
     a.score_len = plan.score_len; a.rows16 = plan.rows16;
     char * w = (char *) ws;
-    if (plan.n_split > 1) a.part = (float *) (w + plan.part);
-    if (plan.n_split > 1 || plan.scored) a.stat = (float2 *) (w + plan.stat);
+    a.units = plan.units;
+    a.most = (a.max_len + 63) / 64;
+    if (plan.units || plan.n_split > 1) a.part = (float *) (w + plan.part);
+    if (plan.units || plan.n_split > 1 || plan.scored) a.stat = (float2 *) (w + plan.stat);
+    if (plan.units) a.split = (int2 *) (w + plan.split);
     if (plan.scored) a.score = (float *) (w + plan.score);
     if (plan.drawn) { a.qh = (uint16_t *) (w + plan.qh); a.rowq = (kv8::f4 *) (w + plan.rowq); }
     if (c->head_dim == 64) launch_attend<64>(a, plan, (hipStream_t) stream);

@@ -312,15 +312,17 @@ struct AttendArgs {
     int64_t qs, qr, qhd, os, orow, oh;
     const int32_t * lens, * n_new;
     int32_t len0, q_type, o_type, n_rows, n_head, group, max_len, causal, weights, qvec, ovec;
-    float scale;
+    float scale, per_group;             // 1 / group
     int32_t split_tiles, n_split;       // 64-slot tiles a split
     int32_t row_tiles;                  // k_attend_tile: row tiles of a sequence and kv head
+    int32_t units, most;                // .. workgroups that their slots are split over (0: not split), tiles at most
     int32_t row_blocks;                 // k_attend_join: workgroups of a sequence and kv head that take rows
     int32_t score_len, rows16;          // scores a row; rows to a multiple of 16
     // workspace, each where the call needs it: [seq][kv head][split][row][D]; [..][row]: maximum, sum; [seq][kv
     // head][row][score_len]; [seq][kv head][rows16][D]: q in fp16; [seq][kv head][rows16]: its factor, the row's
     // maximum, 1 / its sum
     float * part; float2 * stat; float * score; uint16_t * qh; f4 * rowq;
+    int2 * split;                       // k_attend_tile: [seq][kv head][row tile]: its first split, how many
 };
 
 __device__ __forceinline__ int seq_len(const AttendArgs & a, int s) {
@@ -334,6 +336,16 @@ __device__ __forceinline__ int seq_rows(const AttendArgs & a, int s) {
 __device__ __forceinline__ int splits_of(const AttendArgs & a, int slots) {
     return ((slots + 63) / 64 + a.split_tiles - 1) / a.split_tiles;
 }
+// the token of row (token * group + head): rows are under 2^21 and tokens under 2^16, so that the product's error, 2^-23
+// of it, is under half a row's part of a token
+__device__ __forceinline__ int token_of(const AttendArgs & a, int row) {
+    return (int) (((float) row + 0.5f) * a.per_group);
+}
+// where the row's values of a sequence and kv head are in q or out
+__device__ __forceinline__ int64_t row_at(const AttendArgs & a, int row, int g, int64_t per_row, int64_t per_head) {
+    const int tok = token_of(a, row);
+    return tok * per_row + (g * a.group + row - tok * a.group) * per_head;
+}
 // slots that row i sees
 __device__ __forceinline__ int row_limit(const AttendArgs & a, int len, int n, int i) {
     return a.causal ? max(len - n + i + 1, 0) : len;
@@ -343,6 +355,7 @@ __device__ __forceinline__ int row_limit(const AttendArgs & a, int len, int n, i
 typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8v __attribute__((ext_vector_type(8)));
 typedef int i4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 
 // Codes as fp16.  A code's byte with its top bit turned, under the high byte
 // 0x64, is the half 1024 + (code + 128); minus 1152 that is the code, exactly.
@@ -363,41 +376,63 @@ __device__ __forceinline__ uint32_t pack_h(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// One row of q as MFMA operands: this lane's dims off + lo (c % 2) + hi (c / 2) .. + 7 in q[c], in fp16 under the
-// power of two that brings the row's largest value to [1, 2) (exact for fp16, and for all bits of bfloat16 values
-// down to 2^-14 of the largest), with the sign of the scale.  Returns the factor of a product with it (not negative),
-// NaN for a row that is not finite.
+// This lane's dims off + lo (c % 2) + hi (c / 2) .. + 7 of a row of q as they are, all loads at once (a choice of
+// type or alignment at each would wait for each).
 template <int D>
-__device__ __forceinline__ float row_operand(const AttendArgs & a, int64_t at, bool on, int off, int lo, int hi,
-                                             h8v (&q)[D / 32]) {
-    float x[D / 32][8], big = 0.0f, ok = 0.0f;
+__device__ __forceinline__ void load_row(const AttendArgs & a, int64_t at, bool on, int off, int lo, int hi, u4 (&w)[D / 32]) {
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) {
+    for (int c = 0; c < D / 32; ++c) w[c] = (u4){0u, 0u, 0u, 0u};
+    if (!on) return;
+    const uint16_t * p = (const uint16_t *) a.q + at + off;
+    if (a.qvec) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[c][e] = 0.0f;
-        if (on) {
-            if (a.q_type == kF16) load8<kF16>(a.q, at + off + lo * (c & 1) + hi * (c >> 1), a.qvec, x[c]);
-            else load8<kBF16>(a.q, at + off + lo * (c & 1) + hi * (c >> 1), a.qvec, x[c]);
-        }
+        for (int c = 0; c < D / 32; ++c) w[c] = *(const u4 *) (p + lo * (c & 1) + hi * (c >> 1));
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            big = fmaxf(big, fabsf(x[c][e]));
-            ok = fmaf(x[c][e], 0.0f, ok);       // NaN once a value is not finite
-        }
+        for (int c = 0; c < D / 32; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint16_t * y = p + lo * (c & 1) + hi * (c >> 1) + 2 * e;
+                w[c][e] = y[0] | (uint32_t) y[1] << 16;
+            }
     }
-    big = fmaxf(big, __shfl_xor(big, 16));
-    big = fmaxf(big, __shfl_xor(big, 32));
-    ok += __shfl_xor(ok, 16);
-    ok += __shfl_xor(ok, 32);
-    const int ex = big > 0.0f && finite_f(big) ? ilogbf(big) : 0;
+}
+
+// That row as MFMA operands, with the sign of the scale: fp16 as it is; bfloat16 under the power of two that brings
+// the row's largest value to [1, 2) (all bits of values down to 2^-14 of the largest).  Returns the factor of a
+// product with it (not negative), NaN for a row that is not finite.
+template <int D>
+__device__ __forceinline__ float row_operand(const AttendArgs & a, const u4 (&w)[D / 32], h8v (&q)[D / 32]) {
+    const bool half = a.q_type == kF16;
+    us2 most = {0, 0};                          // the largest magnitudes of even and odd dims, as integers
 #pragma unroll
     for (int c = 0; c < D / 32; ++c)
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = ldexpf(x[c][e], -ex);
-            q[c][e] = (_Float16) (a.scale < 0.0f ? -y : y);
+        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, w[c][e] & 0x7fff7fffu));
+    int big = max((int) most[0], (int) most[1]);
+    big = max(big, __shfl_xor(big, 16));
+    big = max(big, __shfl_xor(big, 32));
+    const float ok = big < (half ? 0x7c00 : 0x7f80) ? 0.0f : __uint_as_float(0x7fc00000u);
+    const float scale = fabsf(a.scale) * 1.4426950408889634f;
+    const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+    if (half) {
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) q[c] = __builtin_bit_cast(h8v, w[c] ^ (u4){flip, flip, flip, flip});
+        return scale + ok;
+    }
+    const int ex = min(max(big >> 7, 1), 254) - 127;
+    const float f = ldexpf(1.0f, -ex);
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+        i4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t u = w[c][e] ^ flip;
+            v[e] = (int) pack_h(__uint_as_float(u << 16) * f, __uint_as_float(u & 0xffff0000u) * f);
         }
-    return ldexpf(fabsf(a.scale) * 1.4426950408889634f, ex) + ok;
+        q[c] = __builtin_bit_cast(h8v, v);
+    }
+    return ldexpf(scale, ex) + ok;
 }
 
 // For k_attend_drawn: the row in fp16, and its factor.
@@ -463,7 +498,7 @@ constexpr float kPScale = 16384.0f;    // probabilities enter the value product 
 // Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), four
 // waves; workgroups go to the XCDs in turn, so heads come first and a sequence's splits are turned by its number: the
 // first splits, the only ones of short sequences, spread over all XCDs (16 sequences of 128 to 32,768 slots: 150 us
-// with splits first, 119 so).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with
+// with splits first, 119 so, before a row's loads went out together).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with
 // its own running maximum m and sum, and join at the end.
 //   - S^T = K . Q^T: 16 slots (A, codes straight from memory) by 16 rows (B) an MFMA of 32 dims.  Lane (i = l % 16, k
 //     = l / 16) holds dims 64 c + 16 k .. + 15 of slot i, and after it the scores of slots 4k .. 4k + 3 of row i.
@@ -475,9 +510,9 @@ constexpr float kPScale = 16384.0f;    // probabilities enter the value product 
 //     the largest value scale of the split (vref) and kPScale, so that they neither overflow nor lose bits.
 //   - With several splits each writes m, the sum and its unnormalised rows; k_attend_join puts them together.
 // Bound by memory: those 16 sequences (8 kv heads of 128, 2 rows each, 540 MB) at 4.5 TB/s; 131,001 slots of 4 kv
-// heads of 64 (67 MB) 17 us; 2,049 slots of 8 kv heads 7.8, where it is the chain of a length, a tile and the waves'
+// heads of 64 (67 MB) 16 us; 2,049 slots of 8 kv heads 7.6, where it is the chain of a length, a tile and the waves'
 // join.  The next tile's keys go out when this one's scores are formed, its values when this one's product is: two
-// whole tiles in registers leave one wave a SIMD and take 135 us where this takes 119; 3 waves a SIMD spill (300).
+// whole tiles in registers leave one wave a SIMD and take 135 us where this took 119; 3 waves a SIMD spill (300).
 template <int D, int RT>
 __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
@@ -533,12 +568,20 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
     float qs[RT], m[RT], sum[RT];
     int lim[RT];
     f4 o[RT][NJ];
+    u4 raw[RT][NC];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = min(16 * r + i, rows - 1);
+        load_row<D>(a, s * a.qs + row_at(a, row, g, a.qr, a.qhd), 16 * r + i < rows, 16 * k, 8, 64, raw[r]);
+    }
+    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
+    const float vscale = kPScale / vref;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int row = 16 * r + i;
         const bool on = row < rows;
-        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 16 * k, 8, 64, q[r]);
+        const int tok = token_of(a, row);
+        qs[r] = row_operand<D>(a, raw[r], q[r]);
         if (split == 0 && w == 0) keep_row<D>(a, hd, row, on, k == 0, 16 * k, 8, 64, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
@@ -546,8 +589,6 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
-    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
-    const float vscale = kPScale / vref;
     const int lim_all = row_limit(a, len, n, 0);    // slots that every row sees
     for (int tile = first; tile < t1; tile += 4) {
         f4 sc[RT][4];
@@ -671,14 +712,14 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
                 for (int j = 0; j < NJ; j += 4) *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
             } else {
-                store_out<NJ>(a, s * a.os + at / a.group * a.orow + (g * a.group + at % a.group) * a.oh + d0, y);
+                store_out<NJ>(a, s * a.os + row_at(a, at, g, a.orow, a.oh) + d0, y);
             }
         }
     }
 }
 
 constexpr int kSplitMax = 1024;
-constexpr int kTileT = 256, kTileRows = 128;
+constexpr int kTileT = 256, kTileRows = 128, kUnits = 512;
 
 // acc of 1,024 slots (the blk-th) from the scores that k_attend_few kept; eight rows at most.
 __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
@@ -741,20 +782,30 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     const int64_t hd = (int64_t) s * a.c.n_kv_head + g;
     const int row = MANY ? blockIdx.x : blockIdx.x * GR + gr;
     if (row >= rows) return;                        // MANY: the whole workgroup
-    const int live = splits_of(a, a.row_tiles ? row_limit(a, len, n, (min((row / kTileRows + 1) * kTileRows, rows) - 1) / a.group) : len);
+    int live, step;                                 // splits, and how many rows of the workspace they are apart
+    int64_t cell;
+    if (a.row_tiles) {
+        const int2 z = a.split[hd * a.row_tiles + row / kTileRows];
+        live = z.y;
+        step = a.c.n_kv_head * kTileRows;
+        cell = ((int64_t) z.x * a.c.n_kv_head + g) * kTileRows + row % kTileRows;
+    } else {
+        live = splits_of(a, len);
+        step = all_rows;
+        cell = hd * a.n_split * all_rows + row;
+    }
     if (live <= 1) return;                          // written by its split
-    const int64_t cell = hd * a.n_split * all_rows + row;
     float top = -INFINITY, sum = 0.0f;
     f4 o = {0.f, 0.f, 0.f, 0.f};
     if constexpr (MANY) {
-        for (int x = t; x < live; x += 256) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
+        for (int x = t; x < live; x += 256) top = fmaxf(top, a.stat[cell + (int64_t) x * step].x);
         top = wave_max_f(top);
         if ((t & 63) == 0) red[t >> 6] = top;
         __syncthreads();
         top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         const float base = top == -INFINITY ? 0.0f : top;
         for (int x = t; x < live; x += 256) {
-            const float2 st = a.stat[cell + (int64_t) x * all_rows];
+            const float2 st = a.stat[cell + (int64_t) x * step];
             fac[x] = __builtin_amdgcn_exp2f(st.x - base);
             sum = fmaf(st.y, fac[x], sum);
         }
@@ -764,18 +815,22 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         __syncthreads();
         sum = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll 4
-        for (int x = gr; x < live; x += GR)
-            if (fac[x] != 0.0f) o += *(const f4 *) (a.part + (cell + (int64_t) x * all_rows) * D + 4 * ln) * fac[x];
+        for (int x = gr; x < live; x += GR) {
+            const f4 y = *(const f4 *) (a.part + (cell + (int64_t) x * step) * D + 4 * ln);
+            const float f = fac[x];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = fmaf(f != 0.0f ? y[e] : 0.0f, f, o[e]);  // 0: perhaps never written
+        }
         po[gr][ln] = o;
         __syncthreads();
         if (gr) return;
 #pragma unroll
         for (int x = 1; x < GR; ++x) o += po[x][ln];
     } else {
-        for (int x = 0; x < live; ++x) top = fmaxf(top, a.stat[cell + (int64_t) x * all_rows].x);
+        for (int x = 0; x < live; ++x) top = fmaxf(top, a.stat[cell + (int64_t) x * step].x);
         const float base = top == -INFINITY ? 0.0f : top;
         for (int x = 0; x < live; ++x) {
-            const int64_t at = cell + (int64_t) x * all_rows;
+            const int64_t at = cell + (int64_t) x * step;
             const float2 st = a.stat[at];
             if (st.y == 0.0f) continue;             // saw no slot: its row is not written
             const float f = __builtin_amdgcn_exp2f(st.x - base);
@@ -786,12 +841,71 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
     if (a.rowq && ln == 0) keep_sum(a, hd * a.rows16 + row, top, sum);
     o *= inverse(sum);
     const float y[4] = {o[0], o[1], o[2], o[3]};
-    store_out<4>(a, s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * ln, y);
+    store_out<4>(a, s * a.os + row_at(a, row, g, a.orow, a.oh) + 4 * ln, y);
 }
 
 // ----------------------------------------------- attention of many rows
-// A tile of 128 rows (n_new x group of a sequence and kv head) over a split of its slots, grid (heads and sequences,
-// fastest, so that a head's workgroups share an XCD's L2; row tiles, those with the most slots first; splits), four
+// Which sequence, row tile and split of it workgroup blockIdx.x takes (heads are fastest); false: none.  Lengths are on
+// the device, so the splits are chosen here, by every wave alike: of 63 lengths from the mean (8 tiles at least) on, 1/16
+// octave apart, the shortest with which all row tiles of all sequences make no more than `units` workgroups, or none,
+// and a row tile's splits of one length.  z: a wave's 512 ints of LDS, so many row tiles of sequences at most.
+__device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & s, int & row_tile, int & split, int & splits) {
+    const int l = threadIdx.x & 63, seqs = a.c.n_seq, n_tile = seqs * a.row_tiles, me = blockIdx.x / a.c.n_kv_head;
+    int all = 0;
+    for (int p = l; p < (n_tile + 7) / 8 * 8; p += 64) {
+        int tiles = 0;
+        if (p < n_tile) {
+            const int sq = p % seqs, row0 = (a.row_tiles - 1 - p / seqs) * kTileRows, n = seq_rows(a, sq), rows = n * a.group;
+            const int lim = row_limit(a, seq_len(a, sq), n, token_of(a, min(row0 + kTileRows, rows) - 1));
+            if (row0 < rows) tiles = max(lim + 63, 64) / 64;
+        }
+        z[p] = tiles;
+        all += tiles;
+    }
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    auto count = [](int tiles, float inv) { return (int) ceilf((float) tiles * inv); };
+    const float mean = fmaxf((float) all * a.c.n_kv_head / a.units, 8.0f);
+    const float inv = l == 63 ? 0.5f / a.most : 1.0f / (mean * __builtin_amdgcn_exp2f(l / 16.0f));
+    int n = 0;
+    for (int p = 0; p < n_tile; p += 8) {           // zeros behind the last
+        const i4 x = *(const i4 *) (z + p), y = *(const i4 *) (z + p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) n += count(x[e], inv) + count(y[e], inv);
+    }
+    const float best = __shfl(inv, __builtin_ctzll(__ballot(n * a.c.n_kv_head <= a.units)));
+    int own = 0, c[8], at[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        at[e] = own;
+        c[e] = 8 * l + e < n_tile ? count(z[8 * l + e], best) : 0;
+        own += c[e];
+    }
+    int in = own;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int y = __shfl_up(in, m);
+        if (l >= m) in += y;
+    }
+    const uint64_t past = __ballot(in > me);
+    if (!past) return false;
+    const int lane = __builtin_ctzll(past), rest = me - (in - own);
+    int p = 0;
+    split = splits = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        if (rest >= at[e] && rest < at[e] + c[e]) { p = 8 * l + e; split = rest - at[e]; splits = c[e]; }
+    p = __builtin_amdgcn_readlane(p, lane);
+    split = __builtin_amdgcn_readlane(split, lane);
+    splits = __builtin_amdgcn_readlane(splits, lane);
+    s = p % seqs;
+    row_tile = a.row_tiles - 1 - p / seqs;
+    return true;
+}
+
+// A tile of 128 rows (n_new x group of a sequence and kv head) over a split of its slots, grid (splits as find_split
+// deals them, or heads and sequences, then row tiles; a head's workgroups share an XCD's L2), four
 // waves of 32 rows.  Tiles of 64 slots become fp16 in LDS once for all rows.  Products, softmax and scales as in
 // k_attend_few; here all waves go through the same tiles, with dims in their own order:
 //   K in LDS: [slot][dim] in 16-byte chunks, chunk c of slot t at c ^ (t % (D / 8));
@@ -801,10 +915,12 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 // Two buffers of each: the next tile's codes are on their way from memory while this one's products run, and go to
 // LDS at the end, one barrier a tile.  A wave reads its operands from LDS four at a time, the next four before the
 // MFMAs of these: left to itself the compiler waits for each read alone.
-// Bound by the vector ALU: a wave and tile of 64 MFMAs (1,000 clocks) has 490 vector instructions (2,300 clocks: 32
-// exponentials, 5 more instructions a score, 100 to turn codes into halves), and two waves a SIMD overlap the two in
-// part. 2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 45 us and 12 for the join; 3 x 209 rows over
-// 4,001 to 12,011 slots (41 GFLOP) 104 us.  Measured and not kept: eight waves of 16 rows (115 us: operands are read
+// Bound by issue: a wave and tile of 64 MFMAs (1,000 clocks) has 380 vector instructions (1,900 clocks: 32
+// exponentials, 5 more instructions a score, 100 to turn codes into halves); alone on its SIMD it takes 4,000 clocks,
+// two overlap to 2,500 each.  Beside the tiles a workgroup takes 12,000 clocks, 5 us: its place and length, q, its
+// rows' way out.  2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 48 us and 10 for the join; 3 x 209
+// rows over 4,001 to 12,011 slots (41 GFLOP) 85 us, 104 with splits of one length for all sequences, as long as the
+// longest would need.  Measured and not kept: eight waves of 16 rows (115 us where this took 104: operands are read
 // twice as often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a
 // second form), the next tile's scores beside this tile's exponentials (124: no registers left for operand reads),
 // wave priorities (no change).
@@ -813,18 +929,23 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
     constexpr int RT = 2, NC = D / 32, NJ = D / 16, NCH = D / 8, KT = 64 * D;
     __shared__ __align__(16) uint16_t lds[4 * KT];      // K of even and odd tiles, V of even and odd tiles
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
-    const int heads = a.c.n_kv_head, s = blockIdx.x / heads, g = blockIdx.x % heads;
-    const int row_tile = a.row_tiles - 1 - blockIdx.y, split = blockIdx.z;
+    const int heads = a.c.n_kv_head, g = blockIdx.x % heads;
+    int s = blockIdx.x / heads, row_tile = a.row_tiles - 1 - blockIdx.y, split = 0, splits = 1;
+    if (a.units) {
+        if (!find_split(a, (int *) lds + 512 * w, s, row_tile, split, splits)) return;
+        __syncthreads();                            // the tiles go where lengths were
+    }
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group, row0 = row_tile * kTileRows;
     if (row0 >= rows) return;
     const int64_t hd = (int64_t) s * heads + g;
-    const int lim_top = row_limit(a, len, n, (min(row0 + kTileRows, rows) - 1) / a.group);
-    const int t0 = split * a.split_tiles, t1 = min(t0 + a.split_tiles, (lim_top + 63) / 64);
-    const bool parts = splits_of(a, lim_top) > 1;
-    if (split && t0 >= t1) return;
+    const int tiles = (row_limit(a, len, n, token_of(a, min(row0 + kTileRows, rows) - 1)) + 63) / 64;
+    const int t0 = (int) ((int64_t) split * tiles / splits), t1 = (int) ((int64_t) (split + 1) * tiles / splits);
+    const bool parts = splits > 1;
+    if (a.units && split == 0 && t == 0)
+        a.split[hd * a.row_tiles + row_tile] = make_int2((int) blockIdx.x / heads, splits);
     const bool work = row0 + 16 * RT * w < rows;        // this wave has rows
 
-    const int plain = row_limit(a, len, n, row0 / a.group) / 64;    // tiles before this one need no mask
+    const int plain = row_limit(a, len, n, token_of(a, row0)) / 64;    // tiles before this one need no mask
     const int last = len - 1, last_blk = last / kBlk;
 
     // staging: 32 bytes of a K row, and 4 dims of 8 V rows a thread; of 64 dims half the threads each
@@ -887,12 +1008,20 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
     float qs[RT], m[RT], sum[RT];
     int lim[RT];
     f4 o[RT][NJ];
+    u4 raw[RT][NC];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+        const int row = row0 + 16 * (RT * w + r) + i, there = min(row, rows - 1);
+        load_row<D>(a, s * a.qs + row_at(a, there, g, a.qr, a.qhd), row < rows, 8 * k, 32, 64, raw[r]);
+    }
+    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
+    const float vscale = kPScale / vref;
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         const int row = row0 + 16 * (RT * w + r) + i;
         const bool on = row < rows;
-        const int tok = on ? row / a.group : 0, head = g * a.group + (on ? row % a.group : 0);
-        qs[r] = row_operand<D>(a, s * a.qs + tok * a.qr + head * a.qhd, on, 8 * k, 32, 64, q[r]);
+        const int tok = token_of(a, row);
+        qs[r] = row_operand<D>(a, raw[r], q[r]);
         if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, 64, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
@@ -900,8 +1029,6 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
-    const float vref = top_scale(a.c.vs + s * a.c.scale_seq + g * a.c.scale_head, 4 * t0, min(4 * t1, last_blk + 1), l);
-    const float vscale = kPScale / vref;
     auto step = [&](int tile, auto masked) {
         const int sl = __float_as_int(tile * 4 + (l & 3) <= last_blk ? sr : 0.0f);
         fetch_k(tile + 1);
@@ -1013,31 +1140,47 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
         for (; tile < min(t1, plain); ++tile) step(tile, std::false_type{});
         for (; tile < t1; ++tile) step(tile, std::true_type{});
     }
+    // rows to memory by way of LDS (fp32, 16-byte chunks c of row x at c ^ x; each wave its own 32 rows), 8 dims of a
+    // row a thread: written from where they are they took 4 us, in a choice of type and alignment for each four dims
+    float * mine = (float *) lds + 16 * RT * w * D;
+    const int64_t cell0 = (int64_t) blockIdx.x * kTileRows + 16 * RT * w;     // a split's rows, where there are several
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         sum[r] += __shfl_xor(sum[r], 16);
         sum[r] += __shfl_xor(sum[r], 32);
-        const int row = row0 + 16 * (RT * w + r) + i;
-        if (row >= rows) continue;
-        const int64_t cell = (hd * a.n_split + split) * a.n_rows * a.group + row;
-        if (parts) {
-            if (k == 0) a.stat[cell] = make_float2(m[r], sum[r]);
-            if (sum[r] == 0.0f) continue;
-        } else if (a.rowq && k == 0) {
-            keep_sum(a, hd * a.rows16 + row, m[r], sum[r]);
+        const int x = 16 * r + i, row = row0 + 16 * RT * w + x;
+        if (row < rows && k == 0) {
+            if (parts) a.stat[cell0 + x] = make_float2(m[r], sum[r]);
+            else if (a.rowq) keep_sum(a, hd * a.rows16 + row, m[r], sum[r]);
         }
         const float f = vref / kPScale * (parts ? 1.0f : inverse(sum[r]));
-        const int64_t out = s * a.os + row / a.group * a.orow + (g * a.group + row % a.group) * a.oh + 4 * k;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const f4 x = o[r][j] * f;
-            if (parts) *(f4 *) (a.part + cell * D + 16 * j + 4 * k) = x;
-            else {
-                const float y[4] = {x[0], x[1], x[2], x[3]};
-                store_out<4>(a, out + 16 * j, y);
-            }
-        }
+        for (int j = 0; j < NJ; ++j) *(f4 *) (mine + x * D + (((4 * j + k) ^ (x & (D / 4 - 1))) << 2)) = o[r][j] * f;
     }
+    __syncthreads();
+    auto rows_out = [&](auto store) {
+#pragma unroll 4
+        for (int u = 0; u < RT * D / 32; ++u) {
+            const int at = 64 * u + l, x = at / (D / 8), d0 = at % (D / 8) * 8, row = row0 + 16 * RT * w + x;
+            if (row >= rows) break;
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const f4 z = *(const f4 *) (mine + x * D + (((d0 + e) / 4 ^ (x & (D / 4 - 1))) << 2));
+#pragma unroll
+                for (int b = 0; b < 4; ++b) y[e + b] = z[b];
+            }
+            store(x, row, d0, y);
+        }
+    };
+    if (parts)
+        rows_out([&](int x, int, int d0, const float (&y)[8]) { store8<kF32>(a.part, (cell0 + x) * D + d0, true, y); });
+    else
+        by_type(a.o_type, [&](auto ot) {
+            rows_out([&](int, int row, int d0, const float (&y)[8]) {
+                store8<decltype(ot)::value>(a.o, s * a.os + row_at(a, row, g, a.orow, a.oh) + d0, a.ovec, y);
+            });
+        });
 }
 
 // acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels
@@ -1102,7 +1245,7 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
             const float factor = rq[0], top = rq[1], inv = row < rows ? rq[2] : 0.0f;
             fetch(rt + by);
             if (16 * rt < clear) {
-                const int lim = row_limit(a, len, n, min(row, rows - 1) / a.group);
+                const int lim = row_limit(a, len, n, token_of(a, min(row, rows - 1)));
 #pragma unroll
                 for (int b = 0; b < NB; ++b)
 #pragma unroll

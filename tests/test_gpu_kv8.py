@@ -440,6 +440,25 @@ def test_attend_large_and_sharp(n):
         check_attend(c, q, [192, 50], scale=1e-38)
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_attend_smallest_queries(n):
+    """Rows of fp16's subnormal numbers, and of bfloat16's, under a scale that makes scores of them."""
+    g = gen(n + 90)
+    c = fill(2, 1, 192, 128, g)
+    tiny = (2.0 ** -22 * torch.randn(2, n, 2, 128, generator=g, device="cuda")).half()
+    check_attend(c, tiny, [192, n + 3], scale=2.0 ** 21)
+    check_attend(c, query(2, n, 2, 128, g, torch.bfloat16, 2.0 ** -128), [192, n + 3], scale=2.0 ** 126)
+
+
+def test_attend_most_rows():
+    """65,535 rows of 31 heads: rows find their token and head; all but the last see nothing or little."""
+    g = gen(13)
+    c = fill(1, 1, 32, 64, g)
+    q = torch.randn(1, 65535, 31, 64, generator=g, device="cuda").half()
+    check_attend(c, q, [29])
+    check_attend(c, q, [17], causal=False, weights=False)
+
+
 def test_attend_long():
     """One row over 40,001 slots of 8 heads, and 40 rows over them."""
     g = gen(11)
