@@ -435,15 +435,18 @@ __device__ __forceinline__ float row_operand(const AttendArgs & a, const u4 (&w)
     return ldexpf(scale, ex) + ok;
 }
 
-// For k_attend_drawn: the row in fp16, and its factor.
+// For k_attend_drawn: 16 rows from `row0` on, in fp16 as the operands they are (a lane's 16 bytes side by side), and
+// the factors; zeros for rows past the last.
 template <int D>
-__device__ __forceinline__ void keep_row(const AttendArgs & a, int64_t head, int row, bool on, bool first, int off, int lo, int hi,
-                                         const h8v (&q)[D / 32], float qs) {
-    if (!a.qh || !on) return;
-    const int64_t at = head * a.rows16 + row;
+__device__ __forceinline__ void keep_rows(const AttendArgs & a, int64_t head, int row0, bool on, const h8v (&q)[D / 32], float qs) {
+    if (!a.qh || row0 >= a.rows16) return;
+    const int l = threadIdx.x & 63;
+    const int64_t at = head * a.rows16 + row0;
 #pragma unroll
-    for (int c = 0; c < D / 32; ++c) *(h8v *) (a.qh + at * D + off + lo * (c & 1) + hi * (c >> 1)) = q[c];
-    if (first) a.rowq[at][0] = qs;
+    for (int c = 0; c < D / 32; ++c) *(h8v *) (a.qh + at * D + 512 * c + 8 * l) = q[c];
+    if (l >= 16) return;
+    if (on) a.rowq[at + l][0] = qs;
+    else a.rowq[at + l] = (f4){0.f, 0.f, 0.f, 0.f};
 }
 
 template <int N>
@@ -582,7 +585,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         const bool on = row < rows;
         const int tok = token_of(a, row);
         qs[r] = row_operand<D>(a, raw[r], q[r]);
-        if (split == 0 && w == 0) keep_row<D>(a, hd, row, on, k == 0, 16 * k, 8, 64, q[r], qs[r]);
+        if (split == 0 && w == 0) keep_rows<D>(a, hd, 16 * r, on, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
         sum[r] = 0.0f;
@@ -1022,7 +1025,7 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
         const bool on = row < rows;
         const int tok = token_of(a, row);
         qs[r] = row_operand<D>(a, raw[r], q[r]);
-        if (split == 0) keep_row<D>(a, hd, row, on, k == 0, 8 * k, 32, 64, q[r], qs[r]);
+        if (split == 0) keep_rows<D>(a, hd, row - i, on, q[r], qs[r]);
         lim[r] = on ? row_limit(a, len, n, tok) : 0;
         m[r] = -INFINITY;
         sum[r] = 0.0f;
@@ -1221,18 +1224,17 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
         }
         // the first row that sees slot j0
         const int rt0 = (a.causal ? max(j0 - (len - n), 0) * a.group / 16 : 0) + w % by, rt1 = (rows + 15) / 16;
-        // from this row on a row sees all of these slots: none is masked (a row past the last one has a finite row's
-        // scores)
+        // from this row on a row sees all of these slots: none is masked (a row past the last one has the factor 0)
         const int clear = a.causal ? max(j0 + 63 - (len - n), 0) * a.group : 0;
-        const uint16_t * qb = a.qh + hd * a.rows16 * D;
-        const f4 * rb = a.rowq + hd * a.rows16;
+        const uint16_t * qb = a.qh + hd * a.rows16 * D + 8 * l;
+        const f4 * rb = a.rowq + hd * a.rows16 + i;
         h8v q[NC];
         f4 rq;
         auto fetch = [&](int rt) {
-            const uint32_t at = (uint32_t) min(16 * rt + i, rows - 1);
+            rt = min(rt, rt1 - 1) * 16;
 #pragma unroll
-            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (qb + (at * D + (uint32_t) (off + lo * (c & 1) + 64 * (c >> 1))));
-            rq = rb[at];
+            for (int c = 0; c < NC; ++c) q[c] = *(const h8v *) (qb + (uint32_t) (rt * D + 512 * c));
+            rq = rb[rt];
         };
         if (rt0 < rt1) fetch(rt0);
         for (int rt = rt0; rt < rt1; rt += by) {
@@ -1242,7 +1244,7 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
             for (int c = 0; c < NC; ++c)
 #pragma unroll
                 for (int b = 0; b < NB; ++b) sc[b] = mfma32(kf[b][c], q[c], c ? sc[b] : (f4){0.f, 0.f, 0.f, 0.f});
-            const float factor = rq[0], top = rq[1], inv = row < rows ? rq[2] : 0.0f;
+            const float factor = rq[0], top = rq[1], inv = rq[2];
             fetch(rt + by);
             if (16 * rt < clear) {
                 const int lim = row_limit(a, len, n, token_of(a, min(row, rows - 1)));
