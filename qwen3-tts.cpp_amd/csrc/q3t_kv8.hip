@@ -234,8 +234,9 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
     if (join.x && many) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), join, dim3(256), 0, st, a);
     else if (join.x) hipLaunchKernelGGL((kv8::k_attend_join<D, false>), join, dim3(256), 0, st, a);
     if (p.drawn) {
-        // waves that share a slot tile, where one a tile would leave CUs without work (each loads the tile's keys: 3
-        // x 209 rows over 12,011 slots, 1, 2, 4 waves: 55, 64, 80 us)
+        // waves that share a slot tile, where one a tile would leave CUs without work (each loads the tile's keys; 1, 2
+        // and 4 waves: 3 x 209 rows over 4,001 to 12,011 slots, 1,128 workgroups of one a tile, 37, 43, 57 us; over 12,011
+        // of one sequence, 376, 23, 21, 28; 2,049 rows over their own, 66, 118, 63, 37)
         const int64_t tiles = (a.max_len + 63) / 64, groups = tiles * H * S / 4;
         const int by = rows <= 48 || groups >= 512 ? 1 : groups >= 256 ? 2 : 4;
         hipLaunchKernelGGL(kv8::k_attend_drawn<D>, dim3((unsigned) ((tiles * by + 3) / 4), H, S), dim3(256), 0, st, a, by,

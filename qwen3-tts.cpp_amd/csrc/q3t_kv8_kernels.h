@@ -1189,16 +1189,17 @@ __global__ __launch_bounds__(kTileT, 2) void k_attend_tile(AttendArgs a) {
 // acc of 64 slots: their probabilities of all rows, from rows in fp16 and the rows' sums that the attention kernels
 // left.  Scores as there, bit for bit (the same order of dims: `lo` 8 of k_attend_few, 32 of k_attend_tile), so that
 // none is above its row's maximum; K in registers, the next 16 rows on their way while these are worked on; the sum
-// over rows is one over lanes i, in order of the row tiles.  A second pass over K rather than kept scores, which from
-// 9 rows on are as many bytes as the keys and values.  Bound by the vector ALU (an exponential a score) and, at 3
-// waves a SIMD, by its last turn: 3 x 209 rows over 4,001 to 12,011 slots 54 us; 128 slots a wave need half the row
-// reads, but leave one wave a SIMD: 100.
+// over rows is one over lanes i, then over them by way of LDS, in a fixed order.  A second pass over K rather than kept
+// scores, which from 9 rows on are as many bytes as the keys and values.  Bound by issue (an exponential and four more
+// instructions a score, at 3 waves a SIMD): 3 x 209 rows over 4,001 to 12,011 slots 35 us; 55 with rows in their own
+// order, whose operands are halves of 16 lines a load, and lanes' sums by exchanges; 128 slots a wave need half the
+// row reads, but leave one wave a SIMD (100 where this took 55), 4 waves a SIMD spill (82).
 // grid (slot tiles / 4 * by, kv heads, sequences): `by` (1, 2 or 4) waves take the row tiles of one slot tile in turn
 // and add up in their order.
 template <int D>
 __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int lo) {
     constexpr int NC = D / 32, NB = 4;
-    __shared__ float part[4][64];
+    __shared__ float part[4][64], sums[4][16][68];
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
     const int heads = a.c.n_kv_head, g = blockIdx.y, s = blockIdx.z;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
@@ -1267,13 +1268,12 @@ __global__ __launch_bounds__(256) void k_attend_drawn(AttendArgs a, int by, int 
         }
     }
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) *(f4 *) &sums[w][i][16 * b + 4 * k] = (f4){add[b][0], add[b][1], add[b][2], add[b][3]};
+    __syncthreads();
+    float own = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-#pragma unroll
-            for (int x = 1; x < 16; x <<= 1) add[b][e] += __shfl_xor(add[b][e], x);
-            if (i == 0) part[w][16 * b + 4 * k + e] = add[b][e];
-        }
+    for (int x = 0; x < 16; ++x) own += sums[w][x][l];
+    part[w][l] = own;
     __syncthreads();
     const int j = j0 + l;
     if (w % by || !n || j >= len) return;
