@@ -175,7 +175,7 @@ namespace {
 
 // How a call runs: its kernels, splits and the parts of its workspace (bytes).
 struct AttendPlan {
-    bool few, scored, drawn;
+    bool few, whole, scored, drawn;
     int rt, row_tiles, units, split_tiles, n_split, score_len, rows16;
     int64_t part, stat, split, score, qh, rowq, total;
 };
@@ -185,11 +185,12 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     const int64_t len = a->max_len ? a->max_len : c->n_slots, heads = (int64_t) c->n_seq * c->n_kv_head;
     const int64_t group = a->n_head / c->n_kv_head, rows = a->n_rows * group, tiles = (len + 63) / 64;
     p.few = rows <= 32;
-    p.scored = a->weights && rows <= 8;
-    p.drawn = a->weights && !p.scored;
     int64_t st;
     if (p.few) {
         p.rt = rows <= 16 ? 1 : 2;
+        // short contexts in one workgroup a head, without a join (one row of 8 x 2 heads with weights over 64, 250, 512,
+        // 1,000 slots: 7.4, 8.3, 10.2, 13.7 us; split and joined 10.8, 12.0, 11.2, 11.4)
+        p.whole = tiles <= kv8::kWhole;
         // 4 tiles (one a wave) to 16 a split, so that there are about 1,024 workgroups: four a CU
         st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 16) + 3) & ~(int64_t) 3;
     } else {
@@ -202,7 +203,10 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
         if (p.units == whole) p.units = 0;
         st = tiles;
     }
-    if (p.few) st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
+    if (p.whole) st = tiles;
+    else if (p.few) st = std::max(st, (tiles + kv8::kSplitMax - 1) / kv8::kSplitMax);
+    p.scored = a->weights && rows <= 8 && !p.whole;
+    p.drawn = a->weights && rows > 8;
     p.split_tiles = (int) st;
     p.n_split = (int) ((tiles + st - 1) / st);
     p.score_len = (int) std::min<int64_t>(tiles * 64, INT32_MAX);
@@ -223,8 +227,10 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
     const int rows = a.n_rows * a.group, H = a.c.n_kv_head, S = a.c.n_seq;
     if (p.few) {
         const dim3 grid(H, p.n_split, S);
-        if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((kv8::k_attend_few<D, 2>), grid, dim3(256), 0, st, a);
+        if (p.whole && p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1, 8>), grid, dim3(512), 0, st, a);
+        else if (p.whole) hipLaunchKernelGGL((kv8::k_attend_few<D, 2, 8>), grid, dim3(512), 0, st, a);
+        else if (p.rt == 1) hipLaunchKernelGGL((kv8::k_attend_few<D, 1, 4>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((kv8::k_attend_few<D, 2, 4>), grid, dim3(256), 0, st, a);
     } else {
         hipLaunchKernelGGL(kv8::k_attend_tile<D>, p.units ? dim3(p.units) : dim3(H * S, p.row_tiles), dim3(kv8::kTileT), 0, st, a);
     }

@@ -12,6 +12,7 @@ namespace kv8 {
 
 constexpr int kF32 = 0, kF16 = 1, kBF16 = 30;   // element types (ggml ids)
 constexpr int kBlk = Q3T_KV8_BLOCK;
+constexpr int kWhole = 8;            // tiles of 64 slots that k_attend_few takes in one workgroup
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
@@ -498,7 +499,7 @@ __device__ __forceinline__ float top_scale(const float * vs, int b0, int b1, int
 }
 constexpr float kPScale = 16384.0f;    // probabilities enter the value product times this (fp16's normal range then ends at 2^-28)
 
-// Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), four
+// Rows of one kv head and sequence (n_new x group of them, 16 RT at most), grid (kv heads, splits, sequences), NW
 // waves; workgroups go to the XCDs in turn, so heads come first and a sequence's splits are turned by its number: the
 // first splits, the only ones of short sequences, spread over all XCDs (16 sequences of 128 to 32,768 slots: 150 us
 // with splits first, 119 so, before a row's loads went out together).  A split is split_tiles tiles of 64 slots; the waves take its tiles in turn, each with
@@ -511,15 +512,19 @@ constexpr float kPScale = 16384.0f;    // probabilities enter the value product 
 //     Row i's dims (D / 4) k .. are its outputs.
 //   - Codes are exact in fp16; a key block's scale multiplies its scores, a value block's the probabilities, under
 //     the largest value scale of the split (vref) and kPScale, so that they neither overflow nor lose bits.
-//   - With several splits each writes m, the sum and its unnormalised rows; k_attend_join puts them together.
+//   - With several splits each (four waves) writes m, the sum and its unnormalised rows; k_attend_join puts them
+//     together.  Eight waves take calls for up to kWhole tiles alone, and their weights too.
 // Bound by memory: those 16 sequences (8 kv heads of 128, 2 rows each, 540 MB) at 4.5 TB/s; 131,001 slots of 4 kv
 // heads of 64 (67 MB) 16 us; 2,049 slots of 8 kv heads 7.6, where it is the chain of a length, a tile and the waves'
 // join.  The next tile's keys go out when this one's scores are formed, its values when this one's product is: two
 // whole tiles in registers leave one wave a SIMD and take 135 us where this took 119; 3 waves a SIMD spill (300).
-template <int D, int RT>
-__global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
+template <int D, int RT, int NW>
+__global__ __launch_bounds__(64 * NW) void k_attend_few(AttendArgs a) {
     constexpr int NC = D / 32, NJ = D / 16, LD = D + 4;
-    __shared__ float mo[4][16][LD], mm[4][16], ml[4][16];
+    constexpr bool whole = NW > 4;                  // the only split of its slots: it adds up their weights too
+    __shared__ float mo[NW][16][LD], mm[NW][16], ml[NW][16];
+    __shared__ float kept[whole ? 8 : 1][whole ? kWhole * 64 : 1], tops[8], invs[8];
+    const bool scored = whole && a.weights && a.n_rows * a.group <= 8;
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), l = t & 63, i = l & 15, k = l >> 4;
     const int g = blockIdx.x, s = blockIdx.z, split = (blockIdx.y + s) % a.n_split;
     const int len = seq_len(a, s), n = seq_rows(a, s), rows = n * a.group;
@@ -593,7 +598,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         for (int j = 0; j < NJ; ++j) o[r][j] = (f4){0.f, 0.f, 0.f, 0.f};
     }
     const int lim_all = row_limit(a, len, n, 0);    // slots that every row sees
-    for (int tile = first; tile < t1; tile += 4) {
+    for (int tile = first; tile < t1; tile += NW) {
         f4 sc[RT][4];
 #pragma unroll
         for (int b = 0; b < 4; ++b) {
@@ -613,7 +618,7 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
             ks[b] = __int_as_float(__builtin_amdgcn_readlane(sl, b));
             vs[b] = __int_as_float(__builtin_amdgcn_readlane(sl, 4 + b));
         }
-        if (tile + 4 < t1) fetch_k(tile + 4);
+        if (tile + NW < t1) fetch_k(tile + NW);
         h8v p[RT][2];
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
@@ -628,7 +633,10 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) top = fmaxf(top, sc[r][b][e]);
             }
-            if (sco && 16 * r + i < rows)
+            if (whole && scored && i < rows)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) *(f4 *) &kept[i][tile * 64 + 16 * b + 4 * k] = sc[r][b];
+            if (!whole && sco && 16 * r + i < rows)
 #pragma unroll
                 for (int b = 0; b < 4; ++b)
                     *(f4 *) (sco + (int64_t) (16 * r + i) * a.score_len + tile * 64 + 16 * b + 4 * k) = sc[r][b];
@@ -680,9 +688,9 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
                     for (int r = 0; r < RT; ++r) o[r][4 * d + j] = mfma32(__builtin_bit_cast(h8v, v), p[r][u], o[r][4 * d + j]);
                 }
             }
-        if (tile + 4 < t1) fetch_v(tile + 4);
+        if (tile + NW < t1) fetch_v(tile + NW);
     }
-    // the four waves' rows under their common maximum, added in wave order
+    // the waves' rows under their common maximum, added in wave order
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
         sum[r] += __shfl_xor(sum[r], 16);
@@ -690,7 +698,10 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
         if (r) __syncthreads();
         if (k == 0) { mm[w][i] = m[r]; ml[w][i] = sum[r]; }
         __syncthreads();
-        const float top = fmaxf(fmaxf(mm[0][i], mm[1][i]), fmaxf(mm[2][i], mm[3][i])), base = top == -INFINITY ? 0.0f : top;
+        float top = mm[0][i];
+#pragma unroll
+        for (int x = 1; x < NW; ++x) top = fmaxf(top, mm[x][i]);
+        const float base = top == -INFINITY ? 0.0f : top;
         const float f = __builtin_amdgcn_exp2f(m[r] - base) * (vref / kPScale);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -699,24 +710,45 @@ __global__ __launch_bounds__(256) void k_attend_few(AttendArgs a) {
                 *(f4 *) &mo[w][i][(D / 4) * k + NJ * e + j] = (f4){o[r][j][e], o[r][j + 1][e], o[r][j + 2][e], o[r][j + 3][e]} * f;
         __syncthreads();
         const int row = t >> 4, d0 = (t & 15) * NJ, at = 16 * r + row;
-        const float big = fmaxf(fmaxf(mm[0][row], mm[1][row]), fmaxf(mm[2][row], mm[3][row]));
-        float all = 0.0f;
+        if (row < 16 && at < rows) {
+            float big = mm[0][row], all = 0.0f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) all += ml[x][row] * __builtin_amdgcn_exp2f(mm[x][row] - (big == -INFINITY ? 0.0f : big));
-        if (at < rows) {
+            for (int x = 1; x < NW; ++x) big = fmaxf(big, mm[x][row]);
+#pragma unroll
+            for (int x = 0; x < NW; ++x) all += ml[x][row] * __builtin_amdgcn_exp2f(mm[x][row] - (big == -INFINITY ? 0.0f : big));
             const int64_t cell = (hd * a.n_split + split) * a.n_rows * a.group + at;
             if (a.stat && d0 == 0) a.stat[cell] = make_float2(big, all);
             if (a.rowq && !parts && d0 == 0) keep_sum(a, hd * a.rows16 + at, big, all);
+            if (scored && d0 == 0) {
+                tops[row] = big == -INFINITY ? 0.0f : big;
+                invs[row] = inverse(all);
+            }
             const float inv = parts ? 1.0f : inverse(all);
             float y[NJ];
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) y[j] = (((mo[0][row][d0 + j] + mo[1][row][d0 + j]) + mo[2][row][d0 + j]) + mo[3][row][d0 + j]) * inv;
+            for (int j = 0; j < NJ; ++j) {
+                y[j] = mo[0][row][d0 + j];
+#pragma unroll
+                for (int x = 1; x < NW; ++x) y[j] += mo[x][row][d0 + j];
+                y[j] *= inv;
+            }
             if (parts) {
 #pragma unroll
-                for (int j = 0; j < NJ; j += 4) *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
+                for (int j = 0; j < NJ; j += 4)
+                    *(f4 *) (a.part + cell * D + d0 + j) = (f4){y[j], y[j + 1], y[j + 2], y[j + 3]};
             } else {
                 store_out<NJ>(a, s * a.os + row_at(a, at, g, a.orow, a.oh) + d0, y);
             }
+        }
+    }
+    if (scored) {
+        __syncthreads();
+        float * acc = a.c.acc + s * a.c.acc_seq + g * a.c.acc_head;
+        for (int j = t; j < len; j += 64 * NW) {
+            float add = 0.0f;
+            for (int r = 0; r < rows; ++r)
+                if (kept[r][j] != -INFINITY) add = fmaf(__builtin_amdgcn_exp2f(kept[r][j] - tops[r]), invs[r], add);
+            acc[j] += add;
         }
     }
 }
@@ -854,7 +886,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 // and a row tile's splits of one length.  z: a wave's 512 ints of LDS, so many row tiles of sequences at most.
 __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & s, int & row_tile, int & split, int & splits) {
     const int l = threadIdx.x & 63, seqs = a.c.n_seq, n_tile = seqs * a.row_tiles, me = blockIdx.x / a.c.n_kv_head;
-    int all = 0;
+    float all = 0.0f;
     for (int p = l; p < (n_tile + 7) / 8 * 8; p += 64) {
         int tiles = 0;
         if (p < n_tile) {
@@ -863,13 +895,13 @@ __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & 
             if (row0 < rows) tiles = max(lim + 63, 64) / 64;
         }
         z[p] = tiles;
-        all += tiles;
+        all += (float) tiles;
     }
 #pragma unroll
     for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     auto count = [](int tiles, float inv) { return (int) ceilf((float) tiles * inv); };
-    const float mean = fmaxf((float) all * a.c.n_kv_head / a.units, 8.0f);
+    const float mean = fmaxf(all * a.c.n_kv_head / a.units, 8.0f);
     const float inv = l == 63 ? 0.5f / a.most : 1.0f / (mean * __builtin_amdgcn_exp2f(l / 16.0f));
     int n = 0;
     for (int p = 0; p < n_tile; p += 8) {           // zeros behind the last

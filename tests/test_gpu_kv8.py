@@ -355,6 +355,20 @@ def test_attend_one_row(h, group, d, dtype):
 
 
 @pytest.mark.parametrize("weights", [False, True])
+@pytest.mark.parametrize("n,group,d", [(1, 2, 128), (1, 8, 64), (3, 5, 64), (2, 16, 128)])
+def test_attend_few_rows_in_one_workgroup_or_several(n, group, d, weights):
+    """Sequences up to 512 slots by one workgroup a head, or as far as the call is sized for more by several."""
+    g = gen(n * 10 + group)
+    lens = [0, 1, n, 63, 64, 65, 300, 511, 512, 700]
+    c = fill(len(lens), 2, 1040, d, g, weights=weights)
+    for dtype in T16:
+        q = query(len(lens), n, 2 * group, d, g, dtype)
+        check_attend(c, q, lens, max_len=512)
+        check_attend(c, q, lens, max_len=513)
+        check_attend(c, q, lens, n_new=[n, n, 0, n - 1, n, 1, n, n, n, n])
+
+
+@pytest.mark.parametrize("weights", [False, True])
 @pytest.mark.parametrize("n,h,group,d", [(2, 2, 2, 128), (5, 1, 3, 64), (7, 2, 4, 128), (16, 1, 2, 64), (17, 2, 1, 128), (33, 1, 2, 128),
                                          (64, 2, 2, 64), (70, 1, 5, 128), (129, 1, 2, 128), (200, 2, 1, 64), (3, 1, 32, 64)])
 def test_attend_rows(n, h, group, d, weights):
