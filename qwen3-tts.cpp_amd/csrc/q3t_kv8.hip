@@ -194,12 +194,14 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
         // 4 tiles (one a wave) to 16 a split, so that there are about 1,024 workgroups: four a CU
         st = (std::min<int64_t>(std::max<int64_t>((heads * tiles + 1023) / 1024, 4), 16) + 3) & ~(int64_t) 3;
     } else {
-        // As many workgroups as run at once, two a CU, or splits of 8 tiles if those are fewer: more start a second turn
+        // As many workgroups as run at once, two a CU, or splits of 4 tiles if those are fewer (of 8, 6, 4, 3, 2 tiles: 4 x
+        // 16 rows of one kv head over 7,207 and 21,659 slots, all kernels, 33, 31, 29, 29, 30 us; 64 x 2 of 8 over 2,000 34,
+        // 32, 31, 28, 27; 1,000 x 2 of 8 over their own 50, 48, 51, 51, 53): more start a second turn
         // (512, 640, 768, 1,024: 3 x 209 rows over 4,001 to 12,011 slots 84, 92, 85, 91 us, 2,049 rows over their own
         // 49, 56, 57, 57).
         p.row_tiles = (int) ((rows + kv8::kTileRows - 1) / kv8::kTileRows);
         const int64_t whole = heads * p.row_tiles;
-        p.units = whole < kv8::kUnits ? (int) std::min<int64_t>(kv8::kUnits, whole * ((tiles + 7) / 8)) : 0;
+        p.units = whole < kv8::kUnits ? (int) std::min<int64_t>(kv8::kUnits, whole * ((tiles + kv8::kLeast - 1) / kv8::kLeast)) : 0;
         if (p.units == whole) p.units = 0;
         st = tiles;
     }

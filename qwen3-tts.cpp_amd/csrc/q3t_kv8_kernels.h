@@ -754,7 +754,7 @@ __global__ __launch_bounds__(64 * NW) void k_attend_few(AttendArgs a) {
 }
 
 constexpr int kSplitMax = 1024;
-constexpr int kTileT = 256, kTileRows = 128, kUnits = 512;
+constexpr int kTileT = 256, kTileRows = 128, kUnits = 512, kLeast = 4;
 
 // acc of 1,024 slots (the blk-th) from the scores that k_attend_few kept; eight rows at most.
 __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
@@ -804,7 +804,7 @@ __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
 // The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores
 // were kept; kv heads; sequences): D / 4 lanes a split, many splits of one row (MANY) by 1024 / D groups whose sums
 // are added in order, or a row a group.
-// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 4 splits 12 us, 2 rows of 128
+// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 3 splits 9 us, 2 rows of 128
 // (sequence, head)s and their weights (34 MB of scores and sums) 12.5, 8 rows in 256 splits 5.
 template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
@@ -850,12 +850,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         __syncthreads();
         sum = (red[4] + red[5]) + (red[6] + red[7]);
 #pragma unroll 4
-        for (int x = gr; x < live; x += GR) {
-            const f4 y = *(const f4 *) (a.part + (cell + (int64_t) x * step) * D + 4 * ln);
-            const float f = fac[x];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(f != 0.0f ? y[e] : 0.0f, f, o[e]);  // 0: perhaps never written
-        }
+        for (int x = gr; x < live; x += GR) o += *(const f4 *) (a.part + (cell + (int64_t) x * step) * D + 4 * ln) * fac[x];
         po[gr][ln] = o;
         __syncthreads();
         if (gr) return;
@@ -867,7 +862,6 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
         for (int x = 0; x < live; ++x) {
             const int64_t at = cell + (int64_t) x * step;
             const float2 st = a.stat[at];
-            if (st.y == 0.0f) continue;             // saw no slot: its row is not written
             const float f = __builtin_amdgcn_exp2f(st.x - base);
             o += *(const f4 *) (a.part + at * D + 4 * ln) * f;
             sum = fmaf(st.y, f, sum);
@@ -881,7 +875,7 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 
 // ----------------------------------------------- attention of many rows
 // Which sequence, row tile and split of it workgroup blockIdx.x takes (heads are fastest); false: none.  Lengths are on
-// the device, so the splits are chosen here, by every wave alike: of 63 lengths from the mean (8 tiles at least) on, 1/16
+// the device, so the splits are chosen here, by every wave alike: of 63 lengths from the mean (kLeast tiles at least) on, 1/16
 // octave apart, the shortest with which all row tiles of all sequences make no more than `units` workgroups, or none,
 // and a row tile's splits of one length.  z: a wave's 512 ints of LDS, so many row tiles of sequences at most.
 __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & s, int & row_tile, int & split, int & splits) {
@@ -901,7 +895,7 @@ __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & 
     for (int m = 1; m < 64; m <<= 1) all += __shfl_xor(all, m);
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     auto count = [](int tiles, float inv) { return (int) ceilf((float) tiles * inv); };
-    const float mean = fmaxf(all * a.c.n_kv_head / a.units, 8.0f);
+    const float mean = fmaxf(all * a.c.n_kv_head / a.units, (float) kLeast);
     const float inv = l == 63 ? 0.5f / a.most : 1.0f / (mean * __builtin_amdgcn_exp2f(l / 16.0f));
     int n = 0;
     for (int p = 0; p < n_tile; p += 8) {           // zeros behind the last
@@ -953,7 +947,7 @@ __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & 
 // Bound by issue: a wave and tile of 64 MFMAs (1,000 clocks) has 380 vector instructions (1,900 clocks: 32
 // exponentials, 5 more instructions a score, 100 to turn codes into halves); alone on its SIMD it takes 4,000 clocks,
 // two overlap to 2,500 each.  Beside the tiles a workgroup takes 12,000 clocks, 5 us: its place and length, q, its
-// rows' way out.  2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 48 us and 10 for the join; 3 x 209
+// rows' way out.  2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 48 us and 9 for the join; 3 x 209
 // rows over 4,001 to 12,011 slots (41 GFLOP) 85 us, 104 with splits of one length for all sequences, as long as the
 // longest would need.  Measured and not kept: eight waves of 16 rows (115 us where this took 104: operands are read
 // twice as often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a

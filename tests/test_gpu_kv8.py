@@ -514,7 +514,7 @@ def test_attend_offsets_past_32_bits():
 
 @pytest.mark.parametrize("n", [1, 6, 12, 40, 150])
 def test_attend_whatever_the_workspace_holds(n, monkeypatch):
-    """Ten splits of 8 tiles, the last begun among the rows' own slots, so that some rows see none of it; and one split."""
+    """Many splits, the last of them near the rows' own slots, and one: no part of it is read that was not written."""
     g = gen(n + 60)
     c = fill(1, 1, 5008, 128, g, spread=0.3)
     q = query(1, n, 1, 128, g, torch.float16, 2.0)
