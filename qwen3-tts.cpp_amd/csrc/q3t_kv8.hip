@@ -236,7 +236,9 @@ void launch_attend(kv8::AttendArgs a, const AttendPlan & p, hipStream_t st) {
     } else {
         hipLaunchKernelGGL(kv8::k_attend_tile<D>, p.units ? dim3(p.units) : dim3(H * S, p.row_tiles), dim3(kv8::kTileT), 0, st, a);
     }
-    const bool many = p.few ? p.n_split > 8 : p.units > 8 * H * S * p.row_tiles;
+    // a workgroup a row from 17 splits on (209 x 2 rows of 8 heads in 16 splits: 9.9 us so, 6.5 as a row of several; 32 x 8 of
+    // 4 in 64 splits 6.3, 7.2)
+    const bool many = p.few ? p.n_split > 16 : p.units > (int64_t) 16 * H * S * p.row_tiles;
     a.row_blocks = p.n_split == 1 && !p.units ? 0 : many ? rows : (rows + 1024 / D - 1) / (1024 / D);
     const dim3 join(a.row_blocks + (p.scored ? (a.max_len + 1023) / 1024 : 0), H, S);
     if (join.x && many) hipLaunchKernelGGL((kv8::k_attend_join<D, true>), join, dim3(256), 0, st, a);

@@ -804,7 +804,7 @@ __device__ __forceinline__ void scored_slots(const AttendArgs & a, int blk) {
 // The rows of all splits put together, grid (rows / rows a workgroup, then 1,024 slots' weights each where scores
 // were kept; kv heads; sequences): D / 4 lanes a split, many splits of one row (MANY) by 1024 / D groups whose sums
 // are added in order, or a row a group.
-// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 3 splits 9 us, 2 rows of 128
+// Bound by the splits' rows (512 bytes each): 4,098 rows of 8 kv heads in up to 3 splits 8 us, 2 rows of 128
 // (sequence, head)s and their weights (34 MB of scores and sums) 12.5, 8 rows in 256 splits 5.
 template <int D, bool MANY>
 __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
@@ -857,14 +857,29 @@ __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a) {
 #pragma unroll
         for (int x = 1; x < GR; ++x) o += po[x][ln];
     } else {
-        for (int x = 0; x < live; ++x) top = fmaxf(top, a.stat[cell + (int64_t) x * step].x);
-        const float base = top == -INFINITY ? 0.0f : top;
-        for (int x = 0; x < live; ++x) {
-            const int64_t at = cell + (int64_t) x * step;
-            const float2 st = a.stat[at];
-            const float f = __builtin_amdgcn_exp2f(st.x - base);
-            o += *(const f4 *) (a.part + at * D + 4 * ln) * f;
-            sum = fmaf(st.y, f, sum);
+        // four splits' loads at once; the maximum so far moves with each four
+        for (int x = 0; x < live; x += 4) {
+            float2 st[4];
+            f4 y[4];
+            float most = top;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int64_t at = cell + (int64_t) min(x + u, live - 1) * step;
+                st[u] = a.stat[at];
+                y[u] = *(const f4 *) (a.part + at * D + 4 * ln);
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) most = fmaxf(most, st[u].x);
+            const float base = most == -INFINITY ? 0.0f : most, move = __builtin_amdgcn_exp2f(top - base);
+            o *= move;
+            sum *= move;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const float f = x + u < live ? __builtin_amdgcn_exp2f(st[u].x - base) : 0.0f;
+                o += y[u] * f;
+                sum = fmaf(st[u].y, f, sum);
+            }
+            top = most;
         }
     }
     if (a.rowq && ln == 0) keep_sum(a, hd * a.rows16 + row, top, sum);
@@ -947,7 +962,7 @@ __device__ __forceinline__ bool find_split(const AttendArgs & a, int * z, int & 
 // Bound by issue: a wave and tile of 64 MFMAs (1,000 clocks) has 380 vector instructions (1,900 clocks: 32
 // exponentials, 5 more instructions a score, 100 to turn codes into halves); alone on its SIMD it takes 4,000 clocks,
 // two overlap to 2,500 each.  Beside the tiles a workgroup takes 12,000 clocks, 5 us: its place and length, q, its
-// rows' way out.  2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 48 us and 9 for the join; 3 x 209
+// rows' way out.  2,049 rows over their own slots, 8 x 2 heads of 128 (17 GFLOP) 48 us and 8 for the join; 3 x 209
 // rows over 4,001 to 12,011 slots (41 GFLOP) 85 us, 104 with splits of one length for all sequences, as long as the
 // longest would need.  Measured and not kept: eight waves of 16 rows (115 us where this took 104: operands are read
 // twice as often, and it spills), exponents with the scales folded in (3% faster, but scores past 2^16 then need a
