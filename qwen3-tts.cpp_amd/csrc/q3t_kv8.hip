@@ -211,7 +211,7 @@ AttendPlan plan_attend(const q3t_kv8 * c, const q3t_kv8_attend_args * a) {
     p.drawn = a->weights && rows > 8;
     p.split_tiles = (int) st;
     p.n_split = (int) ((tiles + st - 1) / st);
-    p.score_len = (int) std::min<int64_t>(tiles * 64, INT32_MAX);
+    p.score_len = (int) (tiles * 64);
     p.rows16 = (int) ((rows + 15) / 16 * 16);
     auto take = [&](int64_t bytes) { const int64_t at = p.total; p.total += (bytes + 255) / 256 * 256; return at; };
     const int64_t cells = p.units ? (int64_t) p.units * kv8::kTileRows : heads * p.n_split * rows;

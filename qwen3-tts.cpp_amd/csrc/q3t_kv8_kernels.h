@@ -1346,16 +1346,16 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 
 struct EvictLds {
-    uint32_t hist[256 * 8], total[256], cell[32 * kEvT / 64], sums[kEvT / 64], pick[2];   // hist: a copy for each lane mod 8
+    uint32_t hist[256 * 8], total[256], cell[32 * kEvT / 64], sums[kEvT / 64], pick[3];   // hist: a copy for each lane mod 8
 };
 
 // The kept slots of one head with more than `keep` of them.  The threshold (the want-th largest weight of the slots
-// between sink and recent) is found a byte at a time from the top by counting; then the kept slots are numbered in
-// slot order, of those at the threshold the first ones: counts of 64 slots each by ballots, one prefix sum over them,
-// and the place of each slot by the lanes before it.  R slots a thread at a time (slot base + 1,024 r + thread): if
-// they are all there are, weights are read once.  4 for up to 4,096 slots (2,049 slots: 9 us), else 32 (16 x 8 heads
-// of 9,000 to 32,768 slots: 50 us, bound by one workgroup's chain of four counts; 95 with weights read each time and
-// numbered 1,024 at a time).
+// between sink and recent) is found a byte at a time from the top by counting, until all slots that begin with its bytes
+// are kept; then the kept slots are numbered in slot order, of those at the threshold the first ones: counts of 64 slots
+// each by ballots, one prefix sum over them, and the place of each slot by the lanes before it.  R slots a thread at a
+// time (slot base + 1,024 r + thread), as few as take them all, so that weights are read once: 2 x 8 heads of 600 slots
+// 7.3 us (8.7 with 4), one of 2,049 8.5, 4 x 8 of 8,000 13 (25 with 32), 16 x 8 of 12,000 18 (31 with 32), 16 x 8 of 9,000
+// to 32,768 41 (95 with weights read each time and numbered 1,024 at a time).  Bound by one workgroup's chain of counts.
 template <int R>
 __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, const float * acc, int len, int32_t * kept) {
     constexpr int kAt = R * kEvT;
@@ -1371,8 +1371,9 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
         }
     };
     if (once) read(0);
+    const bool some = a.keep > a.sink + a.recent;   // else sink and recent slots are all
     uint32_t want = (uint32_t) (a.keep - a.sink - a.recent), prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int shift = some ? 24 : -8; shift >= 0; shift -= 8) {
         for (int i = t; i < 256 * 8; i += kEvT) z.hist[i] = 0;
         __syncthreads();
         for (int base = 0; base < len; base += kAt) {
@@ -1406,29 +1407,29 @@ __device__ __forceinline__ void select_slots(const EvictArgs & a, EvictLds & z, 
                 if (above < want && above + c[x] >= want) {
                     z.pick[0] = 255 - 4 * l - x;
                     z.pick[1] = above;
+                    z.pick[2] = c[x];
                 }
                 above += c[x];
             }
         }
         __syncthreads();
-        if (want) {                                 // 0: sink and recent slots are all
-            prefix |= z.pick[0] << shift;
-            want -= z.pick[1];
-        }
+        prefix |= z.pick[0] << shift;
+        want -= z.pick[1];
         mask |= 255u << shift;
+        const bool done = want == z.pick[2];        // all with these bytes are kept
         __syncthreads();
+        if (done) break;
     }
-    // prefix: the threshold; want: how many slots at it are kept
+    // prefix: the threshold, in the bytes of mask (those kept whole end in ones); want: how many slots at it are kept
+    const uint32_t least = some ? max(prefix, 1u) : 0xffffffffu, most = some ? prefix | ~mask : 0xffffffffu;
     uint32_t over = 0, at = 0;                      // kept for sure, and at the threshold, so far
     for (int base = 0; base < len; base += kAt) {
         if (!once) read(base);
-        // of those between sink and recent, the ones above the threshold; none where sink and recent are all
-        const uint32_t least = a.keep > a.sink + a.recent ? prefix : 0xffffffffu;
         auto sure = [&](int r) {
             const int i = base + kEvT * r + t;
-            return key[r] ? key[r] > least : i < len;
+            return key[r] ? key[r] > most : i < len;
         };
-        auto tie = [&](int r) { return key[r] && key[r] == prefix; };
+        auto tie = [&](int r) { return key[r] >= least && key[r] <= most; };
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const uint64_t s = __ballot(sure(r)), e = __ballot(tie(r));
@@ -1481,7 +1482,10 @@ __global__ __launch_bounds__(kEvT) void k_evict_select(EvictArgs a) {
         return;
     }
     const float * acc = a.f.acc + s * a.f.acc_seq + h * a.f.acc_head;
-    if (len <= 4 * kEvT) select_slots<4>(a, z, acc, len, kept);
+    if (len <= kEvT) select_slots<1>(a, z, acc, len, kept);
+    else if (len <= 4 * kEvT) select_slots<4>(a, z, acc, len, kept);
+    else if (len <= 8 * kEvT) select_slots<8>(a, z, acc, len, kept);
+    else if (len <= 16 * kEvT) select_slots<16>(a, z, acc, len, kept);
     else select_slots<32>(a, z, acc, len, kept);
 }
 

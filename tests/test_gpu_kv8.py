@@ -663,6 +663,21 @@ def test_evict_ties(kind):
         check_evict(c, [3001, 2905], keep, 5, 60)
 
 
+@pytest.mark.parametrize("n", [1023, 1025, 4096, 4097, 8192, 8200, 16384, 16390, 32768, 32771])
+@pytest.mark.parametrize("kind", ["any", "close", "coarse"])
+def test_evict_threshold(n, kind):
+    """Lengths around the numbers of slots that a thread takes; weights that part at their first bytes, only at their
+    last, or not at all."""
+    g = gen(n)
+    c = fill(1, 1, -(-n // 16) * 16, 64, g)
+    if kind == "close":
+        c.tensors[4].mul_(2.0 ** -10).add_(1.0)
+    elif kind == "coarse":
+        c.tensors[4].mul_(16.0).round_()
+    check_evict(c, [n], n // 3, 3, n // 7)
+    check_evict(c, [n], n // 3, n // 3 - 20, 20)
+
+
 def test_evict_long_and_views():
     g = gen(6)
     big = fill(1, 4, 70000, 64, g)
