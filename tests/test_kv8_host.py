@@ -91,11 +91,14 @@ def test_attend_refuses_weights_without_acc_and_a_small_workspace():
     lib, b = kv8.load_kv8_library(), ctypes.byref
     refused(lib.q3t_kv8_attend_ws(b(cache(acc=None)), b(attend_args())), "weights")
     assert lib.q3t_kv8_attend_ws(b(cache(acc=None)), b(attend_args(weights=0))) >= 0
-    need = lib.q3t_kv8_attend_ws(b(cache()), b(attend_args()))
+    # one workgroup a head takes up to 512 slots, with no workspace
+    assert lib.q3t_kv8_attend_ws(b(cache()), b(attend_args())) == 0
+    more = cache(n_slots=1024)
+    need = lib.q3t_kv8_attend_ws(b(more), b(attend_args()))
     assert need > 0
-    refused(lib.q3t_kv8_attend(0, b(cache()), b(attend_args()), P, need - 1, None), "workspace")
-    refused(lib.q3t_kv8_attend(0, b(cache()), b(attend_args()), None, need, None), "workspace")
-    refused(lib.q3t_kv8_attend(0, b(cache()), b(attend_args()), P + 4, need, None), "aligned")
+    refused(lib.q3t_kv8_attend(0, b(more), b(attend_args()), P, need - 1, None), "workspace")
+    refused(lib.q3t_kv8_attend(0, b(more), b(attend_args()), None, need, None), "workspace")
+    refused(lib.q3t_kv8_attend(0, b(more), b(attend_args()), P + 4, need, None), "aligned")
 
 
 def test_append_evict_read_refuse():
